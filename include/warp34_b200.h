@@ -488,6 +488,71 @@ int warp34_qsa_sparse_paged_attn_hadamard_f16(const warp34_exec* ex, const void*
                                               int local_q_heads, int select_k_blocks, float sm_scale);
 
 /*
+ * Norm and rotary embedding of every query and key head of packed projection rows, and the split of the layer's output gate, in one
+ * pass (additive; the reference's producer, warp34_cuda.h:264-287, is fp16 only and rounds between its steps).  Per head row
+ * x of 256 values:
+ *   y = x / sqrt(mean(x^2) + rms_eps) * (weight_offset + w)              weight_offset 1: weights stored as w - 1
+ *   y[i], y[i + h] <- y[i] cos a - y[i + h] sin a, y[i + h] cos a + y[i] sin a,  a = position * inv_freq[i],  i < h = rotary_dim / 2
+ * in fp32 with one rounding at the end; angles are reduced exactly, whatever the position (also negative).  What comes out is what
+ * the append of any layer format (warp34_kv_cache_write_strided and its bf16 forms) and the attention entry points take.
+ * Rows of q_in hold num_q_heads x 256 values, or, with gate_out, num_q_heads x [256 query | 256 gate]; the gate is copied as it is.
+ * position_planes 1: positions[token].  3: positions[plane * position_plane_stride + token], frequency i of plane 1 where i % 3 == 1 and
+ * i < 3 mrope_s1, of plane 2 where i % 3 == 2 and i < 3 mrope_s2, of plane 0 otherwise (the sections of
+ * warp34_fused_k_rmsnorm_rope_kv_cache_write_f16).
+ * num_q_heads or num_kv_heads may be 0; the pointers of that half are not looked at then.  Tokens with valid_token_mask == 0 are
+ * skipped, their outputs left untouched.  q_out may be q_in (without a gate) and k_out k_in, with equal strides.  All activations and
+ * weights are fp16 (_f16) or bf16 (_bf16); 2-byte alignment is enough, 16-byte alignment of every row is faster.
+ * head_dim 256 and rotary_dim a multiple of 16 up to 256 (0: no rotation), cudaErrorNotSupported otherwise; no workspace.
+ */
+typedef struct warp34_qk_norm_rope_args {
+    const void* q_in;
+    const void* k_in;
+    void* q_out;
+    void* k_out;
+    void* gate_out;                     /* NULL: rows of q_in hold no gate */
+    const void* q_norm_w;               /* [256] */
+    const void* k_norm_w;               /* [256] */
+    const int32_t* positions;
+    const float* inv_freq;              /* [rotary_dim / 2], radians per position */
+    const uint8_t* valid_token_mask;    /* may be NULL */
+    int64_t q_in_stride;                /* from token to token, in elements; likewise below */
+    int64_t k_in_stride;
+    int64_t q_out_stride;
+    int64_t k_out_stride;
+    int64_t gate_out_stride;
+    int64_t position_plane_stride;
+    int32_t num_tokens;
+    int32_t num_q_heads;
+    int32_t num_kv_heads;
+    int32_t head_dim;
+    int32_t rotary_dim;
+    int32_t position_planes;
+    int32_t mrope_s1;
+    int32_t mrope_s2;
+    float   rms_eps;
+    float   weight_offset;
+} warp34_qk_norm_rope_args;
+
+int warp34_qk_norm_rope_f16(const warp34_exec* ex, const warp34_qk_norm_rope_args* args);
+int warp34_qk_norm_rope_bf16(const warp34_exec* ex, const warp34_qk_norm_rope_args* args);
+
+/*
+ * Cached rows read back as fp16 (_f16) or bf16 (_bf16) values: the inverse of the append (additive; a prefix on its way to another
+ * process, to a layer of another format or to a kernel that takes plain rows).  The batch's tokens name the rows, as for the append:
+ * token t's row is write_slot_mapping[t], or, where that is NULL, position context_lens_before[r] + (t - query_start_loc[r]) of its
+ * request through block_tables (seq_lens_after[r] less the request's tokens where context_lens_before is NULL); tokens
+ * whose mask or request mask is 0, slots < 0 and positions outside the table leave their output rows untouched.  k_out / v_out are
+ * [total_tokens][row stride], heads of 256 values next to each other; one of the two may be NULL.
+ *   TQ4: sign diagonal x WHT-256 of (scale x centroid) / 16;  Q8_0, FP8 E4M3: scale x code;  BF16: the row
+ * computed in fp32 and rounded once.  Layers: TQ4 with the rotation, Q8_0 / FP8 E4M3 (each of K and V) or BF16 without, head_dim 256,
+ * 16-token pages, any strides (8-bit rows 4-byte aligned, the others 2-byte), cudaErrorNotSupported otherwise; no workspace.
+ */
+int warp34_kv_cache_read_f16(const warp34_exec* ex, const warp34_kv_layer_layout* layout, const warp34_attention_batch* batch,
+                             void* k_out, void* v_out, int k_row_stride, int v_row_stride);
+int warp34_kv_cache_read_bf16(const warp34_exec* ex, const warp34_kv_layer_layout* layout, const warp34_attention_batch* batch,
+                              void* k_out, void* v_out, int k_row_stride, int v_row_stride);
+
+/*
  * Bounds-checked build (stand-in for the reference's sanitizer runs of this path,
  * tools/check_cuda_sanitizer.py:77-102).  A library compiled with -DW34_BOUNDS
  * (`python -m warp34_b200.build --bounds` -> libwarp34_b200_bounds.so) range-checks, in every kernel,
@@ -498,7 +563,7 @@ int warp34_qsa_sparse_paged_attn_hadamard_f16(const warp34_exec* ex, const void*
  * (reads) or is skipped (writes); nothing traps.  warp34_bounds_report() fills
  *   out4[0] = what | where << 8   what: 1 block-table index, 2 page id, 3 write slot; 0 = no violation
  *                                 where: 1 append, 2 fp32 attention, 3 decode stream, 4 unused,
- *                                        5 / 6 prefill kernels, 7 bf16 KV, 8 8-bit KV
+ *                                        5 / 6 prefill kernels, 7 bf16 KV, 8 8-bit KV, 9 query-sparse, 10 read
  *   out4[1] = the offending value, out4[2] = its limit     (of the first violation seen)
  *   out4[3] = number of violations since the last reset
  * and clears the record when `reset` is non-zero.  Both calls are blocking copies.  In the regular

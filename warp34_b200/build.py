@@ -21,6 +21,8 @@ COMMON = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC", "-I", INCLUDE
 CUDA_UNITS = [
     ("tq4_append.cu", ["-use_fast_math"]),
     ("tq4_attention.cu", []),
+    ("qk_norm_rope.cu", []),
+    ("kv_read.cu", []),
     ("abi_misc.cu", []),
 ]
 HOST_UNITS = ["page_pool.cpp", "prefix_cache.cpp"]

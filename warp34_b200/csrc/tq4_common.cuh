@@ -129,7 +129,7 @@ static int launch_behind(void (*kernel)(const Params), dim3 grid, unsigned threa
 // warp34_bounds_set_pool_pages().  Without the define these helpers cost nothing.
 enum { kBoundsBlockIndex = 1, kBoundsPageId = 2, kBoundsWriteSlot = 3 };
 enum { kInAppend = 1, kInScalar = 2, kInStream = 3, kInPrefillExact = 5, kInPrefillTc = 6,
-       kInBf16 = 7, kInKv8 = 8, kInSparse = 9 };
+       kInBf16 = 7, kInKv8 = 8, kInSparse = 9, kInRead = 10 };
 #ifdef W34_BOUNDS
 struct BoundsWord { int what, value, limit, count; };
 static __device__ BoundsWord g_bounds;       // one per translation unit; the report merges them

@@ -69,7 +69,17 @@ class PeerMailboxes(C.Structure):
                 ("wait_limit", C.c_uint32), ("reserved", C.c_uint32)]
 
 
-assert C.sizeof(PeerMailboxes) == 168
+class QkNormRopeArgs(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("q_in", "k_in", "q_out", "k_out", "gate_out", "q_norm_w", "k_norm_w", "positions", "inv_freq",
+                                          "valid_token_mask")] + \
+               [(n, C.c_int64) for n in ("q_in_stride", "k_in_stride", "q_out_stride", "k_out_stride", "gate_out_stride",
+                                         "position_plane_stride")] + \
+               [(n, C.c_int32) for n in ("num_tokens", "num_q_heads", "num_kv_heads", "head_dim", "rotary_dim", "position_planes",
+                                         "mrope_s1", "mrope_s2")] + \
+               [("rms_eps", C.c_float), ("weight_offset", C.c_float)]
+
+
+assert C.sizeof(PeerMailboxes) == 168 and C.sizeof(QkNormRopeArgs) == 168
 assert C.sizeof(Exec) == 32 and C.sizeof(KvLayerLayout) == 104 and C.sizeof(AttentionBatch) == 96
 
 _P = C.POINTER
@@ -118,6 +128,10 @@ _KERNEL_SIGS = {
     "warp34_paged_attention_bf16": (C.c_int, [_P(Exec), _P(KvLayerLayout), _P(AttentionBatch),
                                               C.c_void_p, C.c_void_p, C.c_int]),
     "warp34_paged_attention_bf16_scratch_bytes": (C.c_size_t, [_P(KvLayerLayout), _P(AttentionBatch), C.c_int]),
+    "warp34_qk_norm_rope_f16": (C.c_int, [_P(Exec), _P(QkNormRopeArgs)]),
+    "warp34_qk_norm_rope_bf16": (C.c_int, [_P(Exec), _P(QkNormRopeArgs)]),
+    "warp34_kv_cache_read_f16": (C.c_int, [_P(Exec), _P(KvLayerLayout), _P(AttentionBatch), C.c_void_p, C.c_void_p, C.c_int, C.c_int]),
+    "warp34_kv_cache_read_bf16": (C.c_int, [_P(Exec), _P(KvLayerLayout), _P(AttentionBatch), C.c_void_p, C.c_void_p, C.c_int, C.c_int]),
     "warp34_b200_version": (C.c_char_p, []),
 }
 

@@ -472,6 +472,85 @@ class PeerExchange:
         _check(rc, "warp34_paged_attention_exchange_merge_f16")
 
 
+def _require(ok, what):
+    if not ok:
+        raise ValueError(what)
+
+
+def _head_rows(t, dtype, heads, width, what):
+    """Checks that t is [tokens, heads, width] with heads next to each other; returns its token stride."""
+    _require(t.dtype == dtype and t.dim() == 3 and t.shape[2] == width and (heads is None or t.shape[1] == heads),
+             f"{what}: expected {dtype} of shape [tokens, heads, {width}], got {t.dtype} {tuple(t.shape)}")
+    _require((t.stride(2) == 1 or t.numel() == 0) and (t.stride(1) == width or t.shape[1] <= 1), f"{what}: heads must be contiguous")
+    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1] * width)
+
+
+def qk_norm_rope(ex, q, k, q_weight, k_weight, positions, inv_freq, q_out, k_out, gate_out=None, sections=None, eps=1e-6,
+                 weight_offset=1.0, valid_token_mask=None, lib=None):
+    """warp34_qk_norm_rope_f16 / _bf16 (by q's or k's type): the norm and rotary embedding of every query and key head.
+
+    q [tokens, heads, 256], or [tokens, heads, 512] with query and gate of a head next to each other where gate_out is given; k [tokens, kv
+    heads, 256]; either may be None with its weight and output.  Rows may be slices of packed projection rows.  positions: int32
+    [tokens], or [3, tokens] with the mRoPE sections; inv_freq: fp32 [rotary_dim / 2]; None: no rotation."""
+    lib = lib or ffi.kernels()
+    _require(q is not None or k is not None, "qk_norm_rope: neither q nor k")
+    dtype = (q if q is not None else k).dtype
+    _require(dtype in (torch.float16, torch.bfloat16), f"qk_norm_rope: fp16 or bf16 rows, got {dtype}")
+    a = ffi.QkNormRopeArgs()
+    n = (q if q is not None else k).shape[0]
+    for name, x, w, out in (("q", q, q_weight, q_out), ("k", k, k_weight, k_out)):
+        if x is None:
+            continue
+        width = 512 if name == "q" and gate_out is not None else 256
+        stride_in, stride_out = _head_rows(x, dtype, None, width, name), _head_rows(out, dtype, x.shape[1], 256, f"{name}_out")
+        _require(x.shape[0] == n and out.shape[0] == n, f"qk_norm_rope: {name} and {name}_out of {n} tokens")
+        _require(w.dtype == dtype and w.numel() == 256 and w.is_contiguous(), f"{name}_weight: 256 contiguous values of {dtype}")
+        setattr(a, f"{name}_in", x.data_ptr())
+        setattr(a, f"{name}_out", out.data_ptr())
+        setattr(a, f"{name}_norm_w", w.data_ptr())
+        setattr(a, f"{name}_in_stride", stride_in)
+        setattr(a, f"{name}_out_stride", stride_out)
+        setattr(a, "num_q_heads" if name == "q" else "num_kv_heads", x.shape[1])
+    if gate_out is not None:
+        _require(q is not None, "qk_norm_rope: a gate without queries")
+        a.gate_out_stride = _head_rows(gate_out, dtype, q.shape[1], 256, "gate_out")
+        _require(gate_out.shape[0] == n, f"qk_norm_rope: gate_out of {n} tokens")
+        a.gate_out = gate_out.data_ptr()
+    if inv_freq is not None and inv_freq.numel() > 0:
+        _require(inv_freq.dtype == torch.float32 and inv_freq.is_contiguous(), "inv_freq: contiguous fp32")
+        _require(positions.dtype == torch.int32 and positions.shape[-1] == n and positions.dim() in (1, 2) and (n <= 1 or positions.stride(-1) == 1),
+                 f"positions: int32 [{n}] or [3, {n}]")
+        planes = 1 if positions.dim() == 1 else positions.shape[0]
+        _require(planes in (1, 3) and (planes == 1 or sections is not None), "positions: one plane, or three and their sections")
+        a.positions, a.inv_freq, a.rotary_dim, a.position_planes = positions.data_ptr(), inv_freq.data_ptr(), 2 * inv_freq.numel(), planes
+        if planes == 3:
+            a.position_plane_stride, a.mrope_s1, a.mrope_s2 = positions.stride(0), sections[1], sections[2]
+    if valid_token_mask is not None:
+        _require(valid_token_mask.dtype == torch.uint8 and valid_token_mask.numel() == n and valid_token_mask.is_contiguous(),
+                 f"valid_token_mask: uint8 [{n}]")
+        a.valid_token_mask = valid_token_mask.data_ptr()
+    a.num_tokens, a.head_dim, a.rms_eps, a.weight_offset = n, 256, eps, weight_offset
+    fn = lib.warp34_qk_norm_rope_f16 if dtype == torch.float16 else lib.warp34_qk_norm_rope_bf16
+    _check(fn(C.byref(ex.ex), C.byref(a)), "warp34_qk_norm_rope")
+
+
+def kv_cache_read(ex, layer, batch, k_out, v_out, lib=None):
+    """warp34_kv_cache_read_f16 / _bf16 (by the outputs' type): the rows of the batch's tokens read back into k_out / v_out [tokens,
+    heads * 256] (either may be None)."""
+    lib = lib or ffi.kernels()
+    outs = [t for t in (k_out, v_out) if t is not None]
+    _require(outs and all(t.dtype == outs[0].dtype for t in outs) and outs[0].dtype in (torch.float16, torch.bfloat16),
+             "kv_cache_read: fp16 or bf16 outputs of one type")
+    n, cols = batch.desc.total_tokens, layer.layout.local_kv_heads * layer.layout.head_dim
+    for t in outs:
+        _require(t.dim() == 2 and t.shape[0] >= n and t.shape[1] == cols and t.stride(1) == 1, f"kv_cache_read: outputs [{n}, {cols}]")
+    stride = lambda t: 0 if t is None else t.stride(0) if t.shape[0] > 1 else max(t.stride(0), cols)  # noqa: E731
+    ptr = lambda t: None if t is None else t.data_ptr()  # noqa: E731
+    fn = lib.warp34_kv_cache_read_f16 if outs[0].dtype == torch.float16 else lib.warp34_kv_cache_read_bf16
+    _check(fn(C.byref(ex.ex), C.byref(layer.layout), C.byref(batch.desc), ptr(k_out), ptr(v_out), stride(k_out), stride(v_out)),
+           "warp34_kv_cache_read")
+
+
 def kv_page_copy(ex, layer, src_page, dst_page, rows, lib=None):
     lib = lib or ffi.kernels()
     _check(lib.warp34_kv_page_copy(C.byref(ex.ex), C.byref(layer.layout), src_page, dst_page, rows),
