@@ -488,6 +488,40 @@ int warp34_qsa_sparse_paged_attn_hadamard_f16(const warp34_exec* ex, const void*
                                               int local_q_heads, int select_k_blocks, float sm_scale);
 
 /*
+ * Paged attention whose scores are changed before the softmax (additive).  For query token t at position p and key position k, per
+ * q head h:
+ *   s = sm_scale q.k
+ *   s = softcap tanh(s / softcap)                      softcap > 0; 0: scores are not capped
+ *   s = s - distance_slopes[h] |p - k|                 where given
+ * over the keys with first <= k <= last:
+ *   first = the window's first key (batch->sliding_window), or key_begin[t] if that is larger
+ *   last  = p (or the sequence's end, WARP34_ATTN_MASK_SYMMETRIC_WINDOW); where key_end is given, key_end[t] - 1 in its place, the sequence's end at most:
+ *           causality is then the caller's to state
+ * key_begin / key_end hold one position per token of the batch: the start of the token's own document in a packed sequence, the end
+ * of a prefix that its tokens see whole.  They take any value: a token whose range is empty gets a row of zeros.
+ * Everything else is warp34_paged_attention_f16's: batch, masks, strides, scratch (warp34_paged_attention_scored_scratch_bytes for the
+ * full grids; less is served more slowly, none by a row-at-a-time fp32 kernel), accuracy, stream, capture.  Masked rows of attn_out are left untouched.
+ * The _FAST_ATTENTION and _TCGEN05_VERIFY flags change nothing here, _PRECISE_ATTENTION selects the fp32 kernel.
+ * Layers: _f16 TQ4 (any strides), Q8_0 / FP8 E4M3 (K and V each in either); _bf16 BF16 and TQ4; head_dim 256, 16-token pages; anything else
+ * returns cudaErrorNotSupported, and so does a softcap outside [2^-10, 1024] (above, a float is too coarse for the cap itself: 2e-4 of
+ * a weight at 1024).  A softcap below 0 or NaN is invalid.  K or V rows with NaN or infinity reach only the rows that see them (rows
+ * that share a tile with one that does are computed a second time, one by one).
+ */
+typedef struct warp34_score_change {
+    const float*   distance_slopes;    /* [num_q_heads] device, may be NULL */
+    const int32_t* key_begin;          /* [total_tokens] device, may be NULL */
+    const int32_t* key_end;            /* [total_tokens] device, may be NULL */
+    float          softcap;
+    int32_t        reserved;
+} warp34_score_change;
+
+int warp34_paged_attention_scored_f16(const warp34_exec* ex, const warp34_kv_layer_layout* layout, const warp34_attention_batch* batch,
+                                      const warp34_score_change* change, const void* q_in, void* attn_out, int num_q_heads);
+int warp34_paged_attention_scored_bf16(const warp34_exec* ex, const warp34_kv_layer_layout* layout, const warp34_attention_batch* batch,
+                                       const warp34_score_change* change, const void* q_in, void* attn_out, int num_q_heads);
+size_t warp34_paged_attention_scored_scratch_bytes(const warp34_kv_layer_layout* layout, const warp34_attention_batch* batch, int num_q_heads);
+
+/*
  * Norm and rotary embedding of every query and key head of packed projection rows, and the split of the layer's output gate, in one
  * pass (additive; the reference's producer, warp34_cuda.h:264-287, is fp16 only and rounds between its steps).  Per head row
  * x of 256 values:

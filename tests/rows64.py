@@ -81,3 +81,97 @@ def half_step(x, dtype):
     """Half a rounding step of dtype at x, as float64."""
     eps, tiny = torch.finfo(dtype).eps, torch.finfo(dtype).smallest_normal
     return np.maximum(np.abs(x) * eps / 2, tiny * eps / 2)
+
+
+# ---- attention with changed scores, by its definition ----------------------------------------------------------------------
+class Cache:
+    """A layer's pages and their rows on the host, a page table and the metadata of one step."""
+
+    def __init__(self, name, heads, lens, ctx, seed, device="cuda", tail=None, spare=2):
+        from warp34_b200 import kv
+        self.name, self.heads, self.lens, self.ctx = name, heads, list(lens), list(ctx)
+        rng = np.random.default_rng(seed)
+        need = [(c + n + 15) // 16 for c, n in zip(ctx, lens)]
+        pages = sum(need) + spare
+        self.layer = kv.KvLayer(pages, heads, formats=formats(name), device=device)
+        self.table = np.zeros((len(lens), max(max(need), 1)), np.int32)
+        order, at = rng.permutation(pages - 1) + 1, 0
+        for r, n in enumerate(need):
+            self.table[r, :n] = order[at:at + n]
+            at += n
+        self.rows = [random_rows(f, pages * heads * 16, rng).reshape(pages, heads, 16, ROW[f]) for f in NAMES[name]]
+        if tail is not None:      # rows no sequence holds: a byte pattern that stands for NaN in every format
+            held = np.zeros((pages, 16), bool)
+            for r, (c, n) in enumerate(zip(ctx, lens)):
+                pos = np.arange(c + n)
+                held[self.table[r, pos // 16], pos % 16] = True
+            for rows in self.rows:
+                rows[~held[:, None, :].repeat(heads, 1)] = tail
+        self.upload()
+
+    def upload(self):
+        for slab, rows in zip((self.layer.k, self.layer.v), self.rows):
+            slab.copy_(torch.from_numpy(rows.copy()).view(-1))
+
+    def batch(self, device="cuda", **kw):
+        from warp34_b200 import kv
+        starts = np.concatenate([[0], np.cumsum(self.lens)])
+        total = np.asarray(self.ctx) + np.asarray(self.lens)
+        return kv.StepBatch(starts, self.ctx, total, self.table, np.zeros(max(int(starts[-1]), 1), np.int32), self.table.shape[1],
+                            kw.pop("sm_scale", 1.0 / 16.0), device=device, **kw)
+
+    def at(self, r, pos, side):
+        """Index of a row in self.rows[side]: [page, :, offset]."""
+        return self.rows[side][self.table[r, pos // 16], :, pos % 16]
+
+    def sequence(self, r):
+        """K and V of request r, float64 [heads, tokens, 256]."""
+        pos = np.arange(self.ctx[r] + self.lens[r])
+        res = []
+        for side, fmt in enumerate(NAMES[self.name]):
+            rows = self.at(r, pos, side)                                    # [tokens, heads, row]
+            res.append(values(rows.reshape(-1, rows.shape[-1]), fmt).reshape(len(pos), self.heads, 256).transpose(1, 0, 2))
+        return res
+
+
+def scored_attention(cache, q, hq, sm_scale=1.0 / 16.0, softcap=0.0, slopes=None, key_begin=None, key_end=None, window=0, symmetric=False):
+    """float64 outputs [tokens, q heads, 256] and, beside them, what errors are taken of: S = sum_k weight_k |V_k| for errors of weights, which
+    multiply whole rows.  On rotated layers also errors of single rotated coordinates (rounded centroids, products, sums) end in a
+    channel, from all 256 coordinates with the signs of the transform: (1 / 16) sum_c +-e_c, whatever the channel's own V.  With
+    |e_c| <= r A_c, A_c = sum_k weight_k |y_kc|, that is r sqrt(mean A_c^2) in the root mean square over the signs: S has
+    sqrt(mean A_c^2) added there, and a tolerance of r' S holds for r up to a quarter of r' (four standard deviations and more)."""
+    n, g = sum(cache.lens), hq // cache.heads
+    q = np.asarray(q, np.float64).reshape(n, hq, 256)
+    out, size = np.zeros((n, hq, 256)), np.zeros((n, hq, 256))
+    at = 0
+    with np.errstate(all="ignore"):
+        for r, (c, m) in enumerate(zip(cache.ctx, cache.lens)):
+            k, v = cache.sequence(r)
+            rotated = NAMES[cache.name][1] == TQ4
+            y = np.abs((v * SIGNS) @ H / 16) if rotated else None      # the transform is its own inverse
+            key = np.arange(c + m)
+            for t in range(m):
+                p = c + t
+                first = 0 if window <= 0 else max(0, p - window + 1)
+                last = c + m - 1 if symmetric else p
+                if key_begin is not None:
+                    first = max(first, int(key_begin[at + t]))
+                if key_end is not None:
+                    last = min(max(int(key_end[at + t]), 0), c + m) - 1
+                if first > last:
+                    continue
+                span = slice(first, last + 1)
+                for h in range(hq):
+                    s = k[h // g][span] @ q[at + t, h] * sm_scale
+                    if softcap > 0:
+                        s = softcap * np.tanh(s / softcap)
+                    if slopes is not None:
+                        s = s - float(slopes[h]) * np.abs(p - key[span])
+                    w = np.exp(s - s.max())
+                    w /= w.sum()
+                    out[at + t, h] = w @ v[h // g][span]
+                    size[at + t, h] = w @ np.abs(v[h // g][span])
+                    if rotated:
+                        size[at + t, h] += np.sqrt(((w @ y[h // g][span]) ** 2).mean())
+            at += m
+    return out, size

@@ -98,3 +98,50 @@ def test_kv_cache_read_wrapper_checks_what_it_is_given(lib):
                  (t(512, 3).T, None)):
         with pytest.raises(ValueError):
             kv.kv_cache_read(ex, layer, batch, k, v)
+
+
+def _scored_call(lib, layout, fn="f16", hq=8, cap=30.0, scratch=0, change=(), q=4096, out=4096, **kw):
+    b = ffi.AttentionBatch()
+    b.query_start_loc = b.block_tables = b.seq_lens_after = 4096
+    b.num_reqs, b.total_tokens, b.max_blocks_per_req, b.max_q_len, b.max_seq_len, b.sm_scale = 1, 5, 2, 5, 20, 0.0625
+    for name, x in kw.items():
+        setattr(b, name, x)
+    c = ffi.ScoreChange(None, None, None, cap, 0)
+    for name, x in change:
+        setattr(c, name, x)
+    return getattr(lib, f"warp34_paged_attention_scored_{fn}")(C.byref(ffi.Exec()), C.byref(layout), C.byref(b), C.byref(c), q, out, hq)
+
+
+def test_scored_attention(lib):
+    lay = canonical_layout(4)
+    lay.k_base = lay.v_base = 1 << 20
+    call = lambda **kw: _scored_call(lib, lay, **kw)  # noqa: E731
+    nan = float("nan")
+    assert call(total_tokens=0) == 0 and call(total_tokens=-1) == 1
+    assert call(cap=-1.0) == 1 and call(cap=nan) == 1 and call(cap=2000.0) == 801 and call(cap=float("inf")) == 801 and call(cap=1e-5) == 801
+    assert call(hq=0) == 1 and call(hq=6) == 1 and call(num_reqs=0) == 1 and call(query_start_loc=None) == 1 and call(block_tables=None) == 1
+    assert call(seq_lens_after=None) == 1 and call(max_blocks_per_req=0) == 1 and call(sliding_window=-1) == 1 and call(mask_mode=7) == 1
+    assert call(q=4097) == 1 and call(out=4099) == 1 and call(change=[("key_begin", 4098)]) == 1 and call(change=[("distance_slopes", 4097)]) == 1
+    ex, b, c = ffi.Exec(), ffi.AttentionBatch(), ffi.ScoreChange()
+    fn = lib.warp34_paged_attention_scored_f16
+    assert fn(None, C.byref(lay), C.byref(b), C.byref(c), 4096, 4096, 8) == 1 and fn(C.byref(ex), C.byref(lay), C.byref(b), None, 4096, 4096, 8) == 1
+    assert fn(C.byref(ex), C.byref(lay), C.byref(b), C.byref(c), None, 4096, 8) == 1
+    for field, value in (("head_dim", 128), ("block_size", 32), ("k_format", ffi.KV_FORMAT_FP16), ("k_transform", 0), ("v_format", ffi.KV_FORMAT_Q8_0)):
+        lay = canonical_layout(4)
+        lay.k_base = lay.v_base = 1 << 20
+        setattr(lay, field, value)
+        assert call() == 801 and call(fn="bf16") == 801, field
+    for name, fn in (("bf16", "f16"), ("fp8", "bf16"), ("q8", "bf16")):      # activations the layer's format has no kernel for
+        assert _scored_call(lib, kv.KvLayer(2, 4, formats=rows64.formats(name), device="cpu").layout, fn=fn) == 801
+
+
+def test_scored_attention_wrapper_checks_what_it_is_given(lib):
+    layer = kv.KvLayer(2, 2, device="cpu")
+    batch = kv.StepBatch([0, 3], [0], [3], [[1]], [16, 17, 18], 1, 0.0625, device="cpu")
+    ex = type("E", (), {"ex": ffi.Exec()})()
+    good = dict(q=torch.zeros(3, 4, 256, dtype=torch.float16), out=torch.zeros(3, 4, 256, dtype=torch.float16), num_q_heads=4)
+    for change in (dict(q=torch.zeros(3, 4, 256)), dict(out=torch.zeros(3, 4, 256, dtype=torch.bfloat16)), dict(q=torch.zeros(2, 4, 256, dtype=torch.float16)),
+                   dict(out=torch.zeros(3, 256, 4, dtype=torch.float16).transpose(1, 2)), dict(slopes=torch.zeros(3)), dict(slopes=torch.zeros(4, dtype=torch.float64)),
+                   dict(key_begin=torch.zeros(2, dtype=torch.int32)), dict(key_end=torch.zeros(3, dtype=torch.int64))):
+        with pytest.raises(ValueError):
+            kv.paged_attention_scored(ex, layer, batch, **{**good, **change})

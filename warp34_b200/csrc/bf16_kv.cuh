@@ -80,6 +80,7 @@ __global__ void __launch_bounds__(128) kv_cache_write_bf16_kernel(const warp34_k
     }
 }
 
+template <bool SCORED>
 __global__ void __launch_bounds__(kBfWarps * 32, 1) bf16kv_attention_stream_kernel(const StreamParams p) {
     grid_dependency_wait();
     grid_launch_dependents();
@@ -133,14 +134,20 @@ __global__ void __launch_bounds__(kBfWarps * 32, 1) bf16kv_attention_stream_kern
 
         int rmax[2], rmin[2];
         bool rvalid[2];
+        float slope[2] = {0.0f, 0.0f};      // SCORED: of the lane's two rows
+        int q_pos[2] = {0, 0};
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
             const int row = group * kBfRows + gid + 8 * x;
             const int q_off = row / p.gqa;
             rvalid[x] = row < rows_in_req &&
                         (p.batch.valid_token_mask == nullptr || p.batch.valid_token_mask[g.q_start + q_off] != 0);
-            rmax[x] = rvalid[x] ? row_max_kv(p.batch, g, q_off) : -1;
-            rmin[x] = rvalid[x] ? row_min_kv(p.batch, g, q_off) : 0x7fffffff;
+            rmax[x] = rvalid[x] ? row_last_key<SCORED>(p.batch, p.sc, g, q_off) : -1;
+            rmin[x] = rvalid[x] ? row_first_key<SCORED>(p.batch, p.sc, g, q_off) : 0x7fffffff;
+            if (SCORED) {
+                slope[x] = rvalid[x] ? row_slope(p.sc, kv_head * p.gqa + row - q_off * p.gqa) : 0.0f;
+                q_pos[x] = g.ctx_before + q_off;
+            }
         }
         int safe_hi = min(rvalid[0] ? rmax[0] : 0x7fffffff, rvalid[1] ? rmax[1] : 0x7fffffff);
         int safe_lo = max(rvalid[0] ? rmin[0] : 0, rvalid[1] ? rmin[1] : 0);
@@ -228,6 +235,17 @@ __global__ void __launch_bounds__(kBfWarps * 32, 1) bf16kv_attention_stream_kern
             for (int n = 0; n < 2; ++n) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) { sc[n][e] = sacc[n][e] * p.q_scale; msk[n][e] = false; }
+            }
+            if (SCORED) {
+                const float away0 = (float)(q_pos[0] - (kv_base + 2 * tig)), away1 = (float)(q_pos[1] - (kv_base + 2 * tig));
+#pragma unroll
+                for (int n = 0; n < 2; ++n) {
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        sc[n][e] = changed_score(p.sc, sc[n][e], slope[0], away0 - (float)(8 * n + e));
+                        sc[n][2 + e] = changed_score(p.sc, sc[n][2 + e], slope[1], away1 - (float)(8 * n + e));
+                    }
+                }
             }
             if (!full) {
 #pragma unroll
@@ -348,9 +366,10 @@ static int bf16kv_configure() {
     if (rc != 0) return rc;
     if (dev < 0 || dev >= 64) return (int)cudaErrorInvalidDevice;
     if (!done[dev]) {
-        rc = (int)cudaFuncSetAttribute(bf16kv_attention_stream_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       kBfWarps * kBfStages * kBfStageBytes);
-        if (rc != 0) return rc;
+        for (auto* kernel : {bf16kv_attention_stream_kernel<false>, bf16kv_attention_stream_kernel<true>}) {
+            rc = (int)cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kBfWarps * kBfStages * kBfStageBytes);
+            if (rc != 0) return rc;
+        }
         done[dev] = true;
     }
     return 0;
@@ -393,10 +412,31 @@ extern "C" size_t warp34_paged_attention_bf16_scratch_bytes(const warp34_kv_laye
            (size_t)slots * (size_t)(w34::kBfRows * w34::kHeadDim + 2 * w34::kBfRows) * sizeof(float);
 }
 
-extern "C" int warp34_paged_attention_bf16(const warp34_exec* ex, const warp34_kv_layer_layout* layout,
-                                           const warp34_attention_batch* batch, const void* q_in, void* attn_out,
-                                           int num_q_heads) {
-    if (ex == nullptr || !w34::bf16_layout_ok(layout) || batch == nullptr || q_in == nullptr || attn_out == nullptr ||
+namespace w34 {
+// Scored attention over BF16 layers: which kernel serves a call.  The CTA-pair kernel takes chunks (more than 16 query rows per kv head in some
+// request: the stream kernel reads a request's pages once for every 16, the pair kernel once for 256), the stream kernel the rest where
+// the workspace holds the plan, the items and one CTA's partials, the row kernel what neither takes.
+enum Bf16Route { kBf16Rows, kBf16Stream, kBf16Pair };
+static Bf16Route bf16_scored_route(const warp34_exec* ex, const warp34_kv_layer_layout* layout, const warp34_attention_batch* batch, int num_q_heads, int* rc) {
+    if ((ex->flags & WARP34_B200_EXEC_FLAG_PRECISE_ATTENTION) != 0 || !bf16_strides_aligned16(layout)) return kBf16Rows;
+    const int gqa = num_q_heads / layout->local_kv_heads;
+    if (gqa <= kPpCtaRows && (long long)batch->max_q_len * gqa > kBfRows) {
+        *rc = bf16kv_configure();
+        return kBf16Pair;
+    }
+    const long long items = items_bound(layout, batch, num_q_heads, kBfRows);
+    const size_t plan = plan_bytes(batch->num_reqs);
+    const size_t avail = ex->scratch_size > plan ? ex->scratch_size - plan : 0;
+    const long long workers = (long long)(avail / ((size_t)(kBfRows * kHeadDim + 2 * kBfRows) * sizeof(float))) - items;
+    if (ex->scratch_ptr == 0 || (ex->scratch_ptr & 15u) != 0 || workers < kBfWarps || items * (long long)batch->max_blocks_per_req >= 0x7fffffffll) return kBf16Rows;
+    return kBf16Stream;
+}
+}  // namespace w34
+
+namespace w34 {
+static int launch_bf16_attention(const warp34_exec* ex, const warp34_kv_layer_layout* layout, const warp34_attention_batch* batch, const void* q_in,
+                                 void* attn_out, int num_q_heads, const ScoreChange* sc) {
+    if (ex == nullptr || !bf16_layout_ok(layout) || batch == nullptr || q_in == nullptr || attn_out == nullptr ||
         num_q_heads <= 0 || num_q_heads % layout->local_kv_heads != 0 || batch->total_tokens < 0 ||
         batch->num_reqs <= 0 || batch->query_start_loc == nullptr || batch->seq_lens_after == nullptr ||
         batch->block_tables == nullptr || batch->max_blocks_per_req <= 0 || batch->sliding_window < 0 ||
@@ -407,11 +447,22 @@ extern "C" int warp34_paged_attention_bf16(const warp34_exec* ex, const warp34_k
     // Unlike the TQ4 entry point this one has no scratch-free fallback: the caller must pass the
     // split-KV workspace (warp34_paged_attention_bf16_scratch_bytes for the full grid; the
     // persistent grid shrinks to what a smaller workspace holds).
-    if (layout->head_dim != w34::kHeadDim || layout->block_size != w34::kPageTokens ||
-        !w34::bf16_strides_aligned16(layout) || ex->scratch_ptr == 0 || (ex->scratch_ptr & 15u) != 0) {
+    if (layout->head_dim != kHeadDim || layout->block_size != kPageTokens) return (int)cudaErrorNotSupported;
+    if (sc != nullptr) {
+        int rc = 0;
+        const Bf16Route route = bf16_scored_route(ex, layout, batch, num_q_heads, &rc);
+        if (rc != 0) return rc;
+        if (route == kBf16Rows) return launch_scored_rows(ex, layout, batch, *sc, q_in, attn_out, num_q_heads, 1);
+        if (route == kBf16Pair) {
+            const OutputGate none = {nullptr, 0};
+            DeviceInfo* dev = device_info(&rc);
+            if (dev == nullptr) return rc;
+            return launch_prefill_pair<WARP34_KV_FORMAT_BF16, true>(ex, layout, batch, q_in, attn_out, num_q_heads, 1, none, dev->sm_count, 0, *sc);
+        }
+    } else if (!bf16_strides_aligned16(layout) || ex->scratch_ptr == 0 || (ex->scratch_ptr & 15u) != 0) {
         return (int)cudaErrorNotSupported;
     }
-    int rc = w34::bf16kv_configure();
+    int rc = bf16kv_configure();
     if (rc != 0) return rc;
     int dev = 0, sms = 0;
     rc = (int)cudaGetDevice(&dev);
@@ -420,17 +471,17 @@ extern "C" int warp34_paged_attention_bf16(const warp34_exec* ex, const warp34_k
     if (rc != 0) return rc;
 
     const int gqa = num_q_heads / layout->local_kv_heads;
-    const long long items = w34::items_bound(layout, batch, num_q_heads, w34::kBfRows);
+    const long long items = items_bound(layout, batch, num_q_heads, kBfRows);
     if (items * (long long)batch->max_blocks_per_req >= 0x7fffffffll) return (int)cudaErrorNotSupported;
-    const size_t plan = w34::plan_bytes(batch->num_reqs);
-    const size_t slot_bytes = (size_t)(w34::kBfRows * w34::kHeadDim + 2 * w34::kBfRows) * sizeof(float);
+    const size_t plan = plan_bytes(batch->num_reqs);
+    const size_t slot_bytes = (size_t)(kBfRows * kHeadDim + 2 * kBfRows) * sizeof(float);
     const size_t avail = ex->scratch_size > plan ? ex->scratch_size - plan : 0;
     const long long workers = (long long)(avail / slot_bytes) - items;
-    if (workers < w34::kBfWarps) return (int)cudaErrorNotSupported;
+    if (workers < kBfWarps) return (int)cudaErrorNotSupported;
     int grid = sms;
-    if (workers / w34::kBfWarps < grid) grid = (int)(workers / w34::kBfWarps);
+    if (workers / kBfWarps < grid) grid = (int)(workers / kBfWarps);
 
-    w34::StreamParams p;
+    StreamParams p;
     p.og.gate = nullptr;
     p.og.mode = 0;
     p.layout = *layout;
@@ -442,17 +493,104 @@ extern "C" int warp34_paged_attention_bf16(const warp34_exec* ex, const warp34_k
     p.scratch = reinterpret_cast<uint8_t*>((uintptr_t)ex->scratch_ptr);
     p.num_q_heads = num_q_heads;
     p.gqa = gqa;
-    p.num_warps = grid * w34::kBfWarps;
+    p.num_warps = grid * kBfWarps;
     p.max_slots = (int)(p.num_warps + items);
-    p.rows_per_group = w34::kBfRows;
+    p.rows_per_group = kBfRows;
     p.q_scale = batch->sm_scale * 1.4426950408889634f;
     p.natural = 1;
     p.qfrag = nullptr;
     p.q_groups_max = 0;
-    p.smem_bytes = (uint32_t)(w34::kBfWarps * w34::kBfStages * w34::kBfStageBytes);
+    p.smem_bytes = (uint32_t)(kBfWarps * kBfStages * kBfStageBytes);
+    if (sc != nullptr) p.sc = *sc;
     cudaStream_t st = (cudaStream_t)ex->stream;
-    rc = w34::launch_behind(w34::tq4_attention_plan_kernel, 1u, 32, 0, st, p);
-    if (rc == 0) rc = w34::launch_behind(w34::bf16kv_attention_stream_kernel, (unsigned)grid, w34::kBfWarps * 32, p.smem_bytes, st, p);
+    rc = launch_behind(tq4_attention_plan_kernel, 1u, 32, 0, st, p);
+    if (rc == 0) rc = launch_behind(sc != nullptr ? bf16kv_attention_stream_kernel<true> : bf16kv_attention_stream_kernel<false>, (unsigned)grid, kBfWarps * 32, p.smem_bytes, st, p);
     if (rc != 0) return rc;
-    return w34::launch_merge<false>(p, (long long)batch->total_tokens * num_q_heads, st);
+    const long long rows = (long long)batch->total_tokens * num_q_heads;
+    return sc != nullptr ? launch_merge<false, true>(p, rows, st) : launch_merge<false>(p, rows, st);
+}
+}  // namespace w34
+
+extern "C" int warp34_paged_attention_bf16(const warp34_exec* ex, const warp34_kv_layer_layout* layout,
+                                           const warp34_attention_batch* batch, const void* q_in, void* attn_out,
+                                           int num_q_heads) {
+    return w34::launch_bf16_attention(ex, layout, batch, q_in, attn_out, num_q_heads, nullptr);
+}
+
+// ---- scored attention: entry points for every layer format --------------------------------------------
+namespace w34 {
+// Attributes of the SCORED builds, once per device.
+static int scored_configure() {
+    static bool done[64];
+    static std::mutex guard;
+    int dev = 0;
+    int rc = (int)cudaGetDevice(&dev);
+    if (rc != 0) return rc;
+    if (dev < 0 || dev >= 64) return (int)cudaErrorInvalidDevice;
+    std::lock_guard<std::mutex> lock(guard);
+    if (done[dev]) return 0;
+    const DeviceInfo* info = device_info(&rc);
+    if (info == nullptr) return rc;
+    for (auto* kernel : {tq4_attention_stream_exact_kernel<false, kEightRows, true>, tq4_attention_stream_exact_kernel<false, kRowsByPlan, true>}) {
+        rc = (int)cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, info->smem_optin);
+        if (rc != 0) return rc;
+    }
+    rc = (int)cudaFuncSetAttribute(attention_prefill_pair_kernel<WARP34_KV_FORMAT_TQ4, true>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                   (int)PpSmem<WARP34_KV_FORMAT_TQ4>::kBytes);
+    if (rc == 0) rc = (int)cudaFuncSetAttribute(attention_prefill_pair_kernel<WARP34_KV_FORMAT_FP8_E4M3, true>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                (int)PpSmem<WARP34_KV_FORMAT_FP8_E4M3>::kBytes);
+    if (rc == 0) rc = (int)cudaFuncSetAttribute(attention_prefill_pair_kernel<WARP34_KV_FORMAT_Q8_0, true>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                (int)PpSmem<WARP34_KV_FORMAT_Q8_0>::kBytes);
+    if (rc == 0) rc = (int)cudaFuncSetAttribute(attention_prefill_pair_kernel<WARP34_KV_FORMAT_BF16, true>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                (int)PpSmem<WARP34_KV_FORMAT_BF16>::kBytes);
+    if (rc == 0) done[dev] = true;
+    return rc;
+}
+
+static int launch_scored_attention(const warp34_exec* ex, const warp34_kv_layer_layout* layout, const warp34_attention_batch* batch,
+                                   const warp34_score_change* change, const void* q_in, void* attn_out, int num_q_heads, int io_bf16) {
+    if (ex == nullptr || layout == nullptr || batch == nullptr || change == nullptr || q_in == nullptr || attn_out == nullptr || batch->total_tokens < 0 ||
+        num_q_heads <= 0 || layout->local_kv_heads <= 0 || num_q_heads % layout->local_kv_heads != 0) {
+        return (int)cudaErrorInvalidValue;
+    }
+    if (batch->total_tokens == 0) return 0;
+    const bool bf16 = bf16_layout_ok(layout), tq4 = tq4_layout_ok(layout), eight = kv8_attention_layout_ok(layout);
+    if (!(io_bf16 ? bf16 || tq4 : tq4 || eight) || layout->head_dim != kHeadDim || layout->block_size != kPageTokens) return (int)cudaErrorNotSupported;
+    if (batch->num_reqs <= 0 || batch->query_start_loc == nullptr || batch->seq_lens_after == nullptr || batch->block_tables == nullptr ||
+        batch->max_blocks_per_req <= 0 || batch->sliding_window < 0 || layout->k_base == 0 || layout->v_base == 0 ||
+        (((uintptr_t)q_in | (uintptr_t)attn_out) & 1u) != 0u || (((uintptr_t)change->distance_slopes | (uintptr_t)change->key_begin | (uintptr_t)change->key_end) & 3u) != 0u ||
+        (batch->mask_mode != WARP34_ATTN_MASK_CAUSAL && batch->mask_mode != WARP34_ATTN_MASK_SYMMETRIC_WINDOW) || !(change->softcap >= 0.0f)) {
+        return (int)cudaErrorInvalidValue;
+    }
+    if (change->softcap != 0.0f && (change->softcap < kMinSoftcap || change->softcap > kMaxSoftcap)) return (int)cudaErrorNotSupported;
+    const int rc = scored_configure();
+    if (rc != 0) return rc;
+    ScoreChange sc;
+    if (change->softcap != 0.0f) {
+        sc.cap = change->softcap * 1.4426950408889634f;
+        sc.cap_arg = 2.0f / change->softcap;
+    }
+    sc.slopes = change->distance_slopes;
+    sc.key_begin = change->key_begin;
+    sc.key_end = change->key_end;
+    if (bf16) return launch_bf16_attention(ex, layout, batch, q_in, attn_out, num_q_heads, &sc);
+    return launch_attention(ex, layout, batch, q_in, attn_out, nullptr, num_q_heads, io_bf16, -1, nullptr, &sc);
+}
+}  // namespace w34
+
+extern "C" int warp34_paged_attention_scored_f16(const warp34_exec* ex, const warp34_kv_layer_layout* layout, const warp34_attention_batch* batch,
+                                                 const warp34_score_change* change, const void* q_in, void* attn_out, int num_q_heads) {
+    return w34::launch_scored_attention(ex, layout, batch, change, q_in, attn_out, num_q_heads, 0);
+}
+extern "C" int warp34_paged_attention_scored_bf16(const warp34_exec* ex, const warp34_kv_layer_layout* layout, const warp34_attention_batch* batch,
+                                                  const warp34_score_change* change, const void* q_in, void* attn_out, int num_q_heads) {
+    return w34::launch_scored_attention(ex, layout, batch, change, q_in, attn_out, num_q_heads, 1);
+}
+extern "C" size_t warp34_paged_attention_scored_scratch_bytes(const warp34_kv_layer_layout* layout, const warp34_attention_batch* batch, int num_q_heads) {
+    if (layout == nullptr || batch == nullptr || num_q_heads <= 0 || layout->local_kv_heads <= 0) return 0;
+    const size_t quantised = warp34_paged_attention_scratch_bytes(layout, batch, num_q_heads);
+    if (layout->k_format != WARP34_KV_FORMAT_BF16) return quantised;
+    // a BF16 chunk has the pair kernel's parts, which the other bound covers; a decode batch items of 16 rows
+    const size_t rows16 = warp34_paged_attention_bf16_scratch_bytes(layout, batch, num_q_heads);
+    return quantised > rows16 ? quantised : rows16;
 }

@@ -325,7 +325,7 @@ __device__ __forceinline__ uint2 lds64_dep(uint32_t addr, uint32_t token) {
 // SPARSE: the query-sparse lists of warp34_qsa_sparse_paged_attn_f16 (see the TQ4 stream kernel): request r
 // is token r, a unit is four entries of its selected list, lanes 0-3 copy their entry's four rows and leave
 // its first position in 16 bytes behind the stage.
-template <int FMT, int STAGES, bool SPARSE = false>
+template <int FMT, int STAGES, bool SPARSE = false, bool SCORED = false>
 __global__ void __launch_bounds__(kKv8StreamWarps * 32, 1) kv8_attention_stream_kernel(const StreamParams p) {
     using G = Kv8Stage<FMT>;
     constexpr bool FP8 = FMT == WARP34_KV_FORMAT_FP8_E4M3;
@@ -396,14 +396,20 @@ __global__ void __launch_bounds__(kKv8StreamWarps * 32, 1) kv8_attention_stream_
 
         int rmax[2], rmin[2];
         bool rvalid[2];
+        float slope[2] = {0.0f, 0.0f};      // SCORED: of the lane's two rows
+        int q_pos[2] = {0, 0};
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
             const int row = group * kRowsPerGroup + 2 * tig + x;
             const int q_off = row / p.gqa;
             rvalid[x] = row < rows_in_req &&
                         (p.batch.valid_token_mask == nullptr || p.batch.valid_token_mask[g.q_start + q_off] != 0);
-            rmax[x] = rvalid[x] ? row_max_kv(p.batch, g, q_off) : -1;
-            rmin[x] = rvalid[x] ? row_min_kv(p.batch, g, q_off) : 0x7fffffff;
+            rmax[x] = rvalid[x] ? row_last_key<SCORED>(p.batch, p.sc, g, q_off) : -1;
+            rmin[x] = rvalid[x] ? row_first_key<SCORED>(p.batch, p.sc, g, q_off) : 0x7fffffff;
+            if (SCORED) {
+                slope[x] = rvalid[x] ? row_slope(p.sc, kv_head * p.gqa + row - q_off * p.gqa) : 0.0f;
+                q_pos[x] = g.ctx_before + q_off;
+            }
         }
         int safe_hi = min(rvalid[0] ? rmax[0] : 0x7fffffff, rvalid[1] ? rmax[1] : 0x7fffffff);
         int safe_lo = max(rvalid[0] ? rmin[0] : 0, rvalid[1] ? rmin[1] : 0);
@@ -637,6 +643,14 @@ __global__ void __launch_bounds__(kKv8StreamWarps * 32, 1) kv8_attention_stream_
             }
 #pragma unroll
             for (int x = 0; x < 4; ++x) sc[x] *= p.q_scale;
+            if (SCORED) {
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    const float away = (float)(q_pos[c] - (kv_base + key_a));
+                    sc[c] = changed_score(p.sc, sc[c], slope[c], away);
+                    sc[2 + c] = changed_score(p.sc, sc[2 + c], slope[c], away - 4.0f);
+                }
+            }
 
             bool msk[4] = {false, false, false, false};
             if (!full) {
@@ -692,7 +706,15 @@ __global__ void __launch_bounds__(kKv8StreamWarps * 32, 1) kv8_attention_stream_
             uint32_t pb[NB][2], pl[NB][2];
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
-                const float pd[4] = {pr[0] * dva[b], pr[1] * dva[b], pr[2] * dvb[b], pr[3] * dvb[b]};
+                // SCORED: held times kUp, so that the residuals of small weights stay in fp16's range (a scale is about 1/100 of its row's
+                // values; without the factor an output of 0.25 over 317 keys was off by up to 9e-5).  What overflows (V above 60 x 127) ends
+                // non-finite and is computed again.
+                constexpr float kUp = SCORED ? 1024.0f : 1.0f;
+                float pd[4] = {pr[0] * (dva[b] * kUp), pr[1] * (dva[b] * kUp), pr[2] * (dvb[b] * kUp), pr[3] * (dvb[b] * kUp)};
+                if (SCORED && !full) {      // a key that only one of the rows sees: its scales may be NaN to the other
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) if (msk[x]) pd[x] = 0.0f;
+                }
 #pragma unroll
                 for (int x = 0; x < 2; ++x) {
                     const __half2 hi = __floats2half2_rn(pd[2 * x], pd[2 * x + 1]);
@@ -769,6 +791,10 @@ __global__ void __launch_bounds__(kKv8StreamWarps * 32, 1) kv8_attention_stream_
             // m-tile mt: row gid = channel c, row gid + 8 = channel c + 1
             const int vw = FP8 ? vword0 + 16 * (mt >> 2) + ((mt >> 1) & 1) : 16 * (mt >> 2) + vword0 + 8 * ((mt >> 1) & 1);
             const int c = 4 * vw + 2 * (mt & 1);
+            if (SCORED) {
+#pragma unroll
+                for (int x = 0; x < 4; ++x) o[mt][x] *= 1.0f / 1024.0f;
+            }
             *reinterpret_cast<float2*>(stage_o + (2 * tig) * kHeadDim + c) = make_float2(o[mt][0], o[mt][2]);
             *reinterpret_cast<float2*>(stage_o + (2 * tig + 1) * kHeadDim + c) = make_float2(o[mt][1], o[mt][3]);
         }
@@ -838,7 +864,8 @@ static long long kv8_stream_workers(const warp34_exec* ex, const warp34_kv_layer
 // this epilogue.
 static int launch_kv8_stream(const warp34_exec* ex, const warp34_kv_layer_layout* layout,
                              const warp34_attention_batch* batch, const void* q_in, void* attn_out,
-                             int num_q_heads, int io_bf16, bool* taken, const OutputGate* short_og = nullptr) {
+                             int num_q_heads, int io_bf16, bool* taken, const OutputGate* short_og = nullptr,
+                             const ScoreChange* sc = nullptr) {
     *taken = false;
     int rc = 0;
     DeviceInfo* dev = device_info(&rc);
@@ -868,6 +895,16 @@ static int launch_kv8_stream(const warp34_exec* ex, const warp34_kv_layer_layout
                                                  (2u * Kv8Stage<WARP34_KV_FORMAT_FP8_E4M3>::kRunStride + 8u)));
             if (rc != 0) return rc;
             rc = (int)cudaFuncSetAttribute(kv8_attention_stream_kernel<WARP34_KV_FORMAT_Q8_0, kKv8StreamStages>,
+                                           cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                           (int)((uint32_t)(kKv8StreamWarps * kKv8StreamStages) *
+                                                 (2u * Kv8Stage<WARP34_KV_FORMAT_Q8_0>::kRunStride + 8u)));
+            if (rc != 0) return rc;
+            rc = (int)cudaFuncSetAttribute(kv8_attention_stream_kernel<WARP34_KV_FORMAT_FP8_E4M3, kKv8StreamStages, false, true>,
+                                           cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                           (int)((uint32_t)(kKv8StreamWarps * kKv8StreamStages) *
+                                                 (2u * Kv8Stage<WARP34_KV_FORMAT_FP8_E4M3>::kRunStride + 8u)));
+            if (rc != 0) return rc;
+            rc = (int)cudaFuncSetAttribute(kv8_attention_stream_kernel<WARP34_KV_FORMAT_Q8_0, kKv8StreamStages, false, true>,
                                            cudaFuncAttributeMaxDynamicSharedMemorySize,
                                            (int)((uint32_t)(kKv8StreamWarps * kKv8StreamStages) *
                                                  (2u * Kv8Stage<WARP34_KV_FORMAT_Q8_0>::kRunStride + 8u)));
@@ -910,15 +947,16 @@ static int launch_kv8_stream(const warp34_exec* ex, const warp34_kv_layer_layout
             p.tokens_per_req = batch->max_q_len;
             p.max_rows = batch->max_q_len * p.gqa;
         }
+        if (sc != nullptr) p.sc = *sc;
         rc = launch_behind(tq4_attention_plan_kernel, 1u, 32, 0, st, p);
         if (rc != 0) return rc;
-        if (fp8) {
-            rc = launch_behind(kv8_attention_stream_kernel<WARP34_KV_FORMAT_FP8_E4M3, kKv8StreamStages>, (unsigned)grid, kKv8StreamWarps * 32, smem, st, p);
-        } else {
-            rc = launch_behind(kv8_attention_stream_kernel<WARP34_KV_FORMAT_Q8_0, kKv8StreamStages>, (unsigned)grid, kKv8StreamWarps * 32, smem, st, p);
-        }
+        auto* kernel = fp8 ? (sc != nullptr ? kv8_attention_stream_kernel<WARP34_KV_FORMAT_FP8_E4M3, kKv8StreamStages, false, true>
+                                            : kv8_attention_stream_kernel<WARP34_KV_FORMAT_FP8_E4M3, kKv8StreamStages>)
+                           : (sc != nullptr ? kv8_attention_stream_kernel<WARP34_KV_FORMAT_Q8_0, kKv8StreamStages, false, true>
+                                            : kv8_attention_stream_kernel<WARP34_KV_FORMAT_Q8_0, kKv8StreamStages>);
+        rc = launch_behind(kernel, (unsigned)grid, kKv8StreamWarps * 32, smem, st, p);
         const long long rows = (short_og != nullptr ? (long long)reqs * batch->max_q_len : (long long)p.batch.total_tokens) * num_q_heads;
-        if (rc == 0) rc = launch_merge<false>(p, rows, st);
+        if (rc == 0) rc = sc != nullptr ? launch_merge<false, true>(p, rows, st) : launch_merge<false>(p, rows, st);
         if (rc != 0) return rc;
         rc = (int)cudaGetLastError();
         if (rc != 0) return rc;

@@ -74,6 +74,11 @@ template <> struct PpFormat<WARP34_KV_FORMAT_Q8_0> {
     static constexpr bool kRotated = false;
     static __device__ __forceinline__ bool has_keys(float l) { return l > 0.0f; }
 };
+template <> struct PpFormat<WARP34_KV_FORMAT_BF16> {      // scored attention only
+    static constexpr uint32_t kRow = 2 * kHeadDim;
+    static constexpr bool kRotated = false;
+    static __device__ __forceinline__ bool has_keys(float l) { return l > 0.0f; }
+};
 
 // A row's scales, as bits: non-negative floats order like them.
 template <int FMT> struct PpScales {
@@ -99,30 +104,34 @@ template <int FMT> struct PpScales {
 };
 __device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
 
+// BF16 rows are operands as they are: no residual parts, no raw stages (the producers copy rows straight into the tiles), more stages.
 template <int FMT> struct PpSmem {
+    static constexpr bool kDirect = FMT == WARP34_KV_FORMAT_BF16;
+    static constexpr int kStages = kDirect ? 8 : kPpStages;
+    static constexpr uint32_t kStage = kDirect ? kPpPart : kPpStage;
     static constexpr uint32_t kRun = kPageTokens * PpFormat<FMT>::kRow;      // one (page, head) run
-    static constexpr uint32_t kRawK = 2u * kRun, kRawV = 4u * kRun;
+    static constexpr uint32_t kRawK = kDirect ? 0u : 2u * kRun, kRawV = kDirect ? 0u : 4u * kRun;
     static constexpr uint32_t kRaw = kRawK + kRawV;
     static constexpr uint32_t kOffK = 0;
-    static constexpr uint32_t kOffV = kOffK + kPpStages * kPpStage;
-    static constexpr uint32_t kOffQLo = kOffV + kPpStages * kPpStage;
+    static constexpr uint32_t kOffV = kOffK + kStages * kStage;
+    static constexpr uint32_t kOffQLo = kOffV + kStages * kStage;
     static constexpr uint32_t kOffRaw = kOffQLo + (PpFormat<FMT>::kRotated ? kPpQLoBytes : 0u);
-    static constexpr uint32_t kOffLut = (kOffRaw + kPpRawStages * kRaw + 127u) & ~127u;
+    static constexpr uint32_t kOffLut = kDirect ? (uint32_t)kPpCtaRows * kPpOutStride * 4u : (kOffRaw + kPpRawStages * kRaw + 127u) & ~127u;
     static constexpr uint32_t kOffBars = kOffLut + (PpFormat<FMT>::kRotated ? kPpLutBytes : 0u);
-    static constexpr uint32_t kBytes = kOffBars + 288u;
+    static constexpr uint32_t kWords = kDirect ? 384u : 224u;      // words behind the barriers, from kOffBars
+    static constexpr uint32_t kBytes = kOffBars + kWords + 64u;
+    static_assert(kOffRaw <= kOffLut, "stages end before what follows them");
     static_assert(kPpCtaRows * kPpOutStride * 4 <= (int)kOffLut, "epilogue staging must end before the table");
     static_assert(kPpCtaRows * 512 <= (int)kOffQLo, "Q' staging fits the tile stages");
     static_assert(!PpFormat<FMT>::kRotated || (kPpCtaRows / 4 + kPpWarps) * 2048 <= (int)kOffQLo, "so do the rows that change lanes behind it");
     static_assert(kBytes <= 227u * 1024u, "shared memory");
+    // barrier slots (8 bytes each).  Full / PReady: waited for by the MMA warp of CTA 0, arrivals from both CTAs.
+    // Empty, S, Pv: one arrival per CTA from the MMA warp's commits.  Raw*: within a CTA.
+    enum { FullK = 0, FullV = FullK + kStages, EmptyK = FullV + kStages, EmptyV = EmptyK + kStages, SReady = EmptyV + kStages, PReady = SReady + 2,
+           Pv = PReady + 2, Drain = Pv + 2, RawKFull, RawKFree = RawKFull + kPpRawStages, RawVFull = RawKFree + kPpRawStages,
+           RawVFree = RawVFull + kPpRawStages, BarCount = RawVFree + kPpRawStages };
+    static_assert((uint32_t)BarCount * 8u <= kWords, "barrier slots end before the words behind them");
 };
-
-// barrier slots (8 bytes each).  Full / PReady: waited for by the MMA warp of CTA 0, arrivals from both CTAs.
-// Empty, S, Pv: one arrival per CTA from the MMA warp's commits.  Raw*: within a CTA.
-enum { kPpFullK = 0, kPpFullV = kPpFullK + kPpStages, kPpEmptyK = kPpFullV + kPpStages, kPpEmptyV = kPpEmptyK + kPpStages,
-       kPpS = kPpEmptyV + kPpStages, kPpPReady = kPpS + 2, kPpPv = kPpPReady + 2, kPpDrain = kPpPv + 2, kPpRawKFull,
-       kPpRawKFree = kPpRawKFull + kPpRawStages, kPpRawVFull = kPpRawKFree + kPpRawStages,
-       kPpRawVFree = kPpRawVFull + kPpRawStages, kPpBarCount = kPpRawVFree + kPpRawStages };
-static_assert(kPpBarCount * 8 <= 224, "barrier slots end before the words behind them");
 
 // ---- CTA-pair wrappers ------------------------------------------------------------------------
 __device__ __forceinline__ uint32_t cluster_rank() {
@@ -207,7 +216,25 @@ struct PrefillPairParams {
     int splits;
     float* parts;
     float2* parts_ml;
+    ScoreChange sc = {};   // SCORED builds
 };
+
+// A pair of operand values in the format's operand type, and back.
+template <int FMT>
+__device__ __forceinline__ uint32_t pp_pack(float a, float b) {
+    if (FMT != WARP34_KV_FORMAT_BF16) return pack_half2(a, b);
+    const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+template <int FMT>
+__device__ __forceinline__ float2 pp_unpack(uint32_t w) {
+    if (FMT != WARP34_KV_FORMAT_BF16) return __half22float2(*reinterpret_cast<const __half2*>(&w));
+    return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+// 16 bytes into shared memory; zeros where `there` is false (nothing is read then).
+__device__ __forceinline__ void pp_copy16(uint32_t dst, const void* src, bool there) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
+}
 
 // ---- rotation of a tile's rows, four at a time -------------------------------------------------------
 // Eight lanes hold a row, 32 columns each, so that five of the eight levels of the 256-point transform are register arithmetic; between two
@@ -294,6 +321,26 @@ __device__ __forceinline__ void prefill_finish_row(const PrefillPairParams& p, f
     store8(p.attn_out, row_base, lane, p.io_bf16, v);
 }
 
+// The same without a gate, for scored attention: a row that is not finite is computed again by itself.
+template <bool ROT>
+__device__ __forceinline__ void prefill_finish_scored_row(const PrefillPairParams& p, float (&v)[8], float l, int req, int q_off, int q_head, int lane) {
+    const float inv = l != 0.0f ? 1.0f / (ROT ? l * (kPpLutScale * 16.0f) : l) : 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] *= inv;
+    if (ROT) {
+        butterfly8<5>(v, lane);
+        sign8(v, lane);
+    }
+    bool fine = is_finite(l);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) fine = fine && is_finite(v[i]);
+    if (!__all_sync(0xffffffffu, fine)) {
+        const ScoredRow one = {&p.layout, &p.batch, &p.sc, p.q_in, p.io_bf16, p.num_q_heads, p.gqa};
+        scored_row_whole(one, req, q_off, q_head, v);
+    }
+    store8(p.attn_out, ((size_t)(p.batch.query_start_loc[req] + q_off) * p.num_q_heads + q_head) * kHeadDim, lane, p.io_bf16, v);
+}
+
 // One query row over its keys in [lo, hi] in fp32 by one warp, as the attention kernel leaves it (columns [8 lane, + 8) of the accumulator,
 // mass, maximum): for tiles whose rows differ so much in magnitude that those the exponents were chosen by are not the others' kind.
 template <int FMT>
@@ -360,8 +407,8 @@ __device__ __forceinline__ void prefill_row_fp32(const PrefillPairParams& p, int
 }
 
 // Combines the splits of every row that takes part: one warp per (token, q head).
-template <bool ROT>
-__global__ void __launch_bounds__(128) prefill_merge_kernel(const PrefillPairParams p) {
+template <bool ROT, bool SCORED = false>
+__global__ void __launch_bounds__(128) prefill_merge_kernel(const __grid_constant__ PrefillPairParams p) {
     grid_dependency_wait();
     grid_launch_dependents();
     const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
@@ -377,7 +424,7 @@ __global__ void __launch_bounds__(128) prefill_merge_kernel(const PrefillPairPar
     if (p.batch.valid_req_mask != nullptr && p.batch.valid_req_mask[r] == 0) return;
     float2 ml = make_float2(-1e30f, 0.0f);
     if (lane < p.splits) ml = p.parts_ml[(size_t)lane * rows + row];
-    const bool part = ROT ? !(ml.y <= 0.0f) : ml.y > 0.0f;      // PpFormat::has_keys
+    const bool part = SCORED ? ml.y != 0.0f : ROT ? !(ml.y <= 0.0f) : ml.y > 0.0f;      // PpFormat::has_keys
     float m_tot = part ? ml.x : -1e30f;
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) m_tot = fmaxf(m_tot, __shfl_xor_sync(0xffffffffu, m_tot, d));
@@ -394,14 +441,22 @@ __global__ void __launch_bounds__(128) prefill_merge_kernel(const PrefillPairPar
         v[0] += ws * a.x; v[1] += ws * a.y; v[2] += ws * a.z; v[3] += ws * a.w;
         v[4] += ws * b.x; v[5] += ws * b.y; v[6] += ws * b.z; v[7] += ws * b.w;
     }
-    prefill_finish_row<ROT>(p, v, l_tot, (size_t)row * kHeadDim, lane);
+    if constexpr (SCORED) prefill_finish_scored_row<ROT>(p, v, l_tot, r, tok - p.batch.query_start_loc[r], (int)(row % p.num_q_heads), lane);
+    else prefill_finish_row<ROT>(p, v, l_tot, (size_t)row * kHeadDim, lane);
 }
 
-template <int FMT>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPpThreads, 1) attention_prefill_pair_kernel(const PrefillPairParams p) {
+// SCORED: scores are changed as score_change.cuh says, P is made from the changed ones, and a row that ends non-finite is computed
+// again by itself.
+template <int FMT, bool SCORED = false>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPpThreads, 1) attention_prefill_pair_kernel(const __grid_constant__ PrefillPairParams p) {
     using S = PpSmem<FMT>;
     constexpr bool ROT = PpFormat<FMT>::kRotated;
     constexpr uint32_t ROW = PpFormat<FMT>::kRow;
+    constexpr bool DIRECT = S::kDirect;
+    constexpr int kPpFullK = S::FullK, kPpFullV = S::FullV, kPpEmptyK = S::EmptyK, kPpEmptyV = S::EmptyV, kPpS = S::SReady, kPpPReady = S::PReady,
+                  kPpPv = S::Pv, kPpDrain = S::Drain, kPpRawKFull = S::RawKFull, kPpRawKFree = S::RawKFree, kPpRawVFull = S::RawVFull,
+                  kPpRawVFree = S::RawVFree;
+    static_assert(!DIRECT || SCORED, "BF16 rows: scored attention");
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
     const uint32_t rank = cluster_rank();
@@ -410,13 +465,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPpThreads, 1) atten
 
     const uint32_t k_t = base + S::kOffK, v_t = base + S::kOffV, qlo_t = base + S::kOffQLo;
     const uint32_t raw = base + S::kOffRaw, lut = base + S::kOffLut, bars = base + S::kOffBars;
-    volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(gen + S::kOffBars + 240);
-    volatile uint32_t* abort_flag = reinterpret_cast<volatile uint32_t*>(gen + S::kOffBars + 244);
-    uint32_t* row_max = reinterpret_cast<uint32_t*>(gen + S::kOffBars + 224);                      // largest scale of the tile's K, V rows
-    volatile int* exponents = reinterpret_cast<volatile int*>(gen + S::kOffBars + 232);            // of K, of V
+    volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(gen + S::kOffBars + S::kWords + 16);
+    volatile uint32_t* abort_flag = reinterpret_cast<volatile uint32_t*>(gen + S::kOffBars + S::kWords + 20);
+    uint32_t* row_max = reinterpret_cast<uint32_t*>(gen + S::kOffBars + S::kWords);                      // largest scale of the tile's K, V rows
+    volatile int* exponents = reinterpret_cast<volatile int*>(gen + S::kOffBars + S::kWords + 8);            // of K, of V
     // request, first block, first token, rows, first token of the request: for the epilogue, which reads them again so that they take no
     // registers from the consumers
-    volatile int* place = reinterpret_cast<volatile int*>(gen + S::kOffBars + 256);
+    volatile int* place = reinterpret_cast<volatile int*>(gen + S::kOffBars + S::kWords + 32);
     auto bar = [&](int which) { return bars + 8u * (uint32_t)which; };
     // Waits and abort checks are warp-uniform: no lane leaves a loop alone.
     auto wait_all = [&](uint32_t b, uint32_t parity) {
@@ -442,7 +497,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPpThreads, 1) atten
         }
     }
     if (tid == 0) {
-        for (int s = 0; s < kPpStages; ++s) {
+        for (int s = 0; s < S::kStages; ++s) {
             mbar_init(bar(kPpFullK + s), 8u);      // four producer warps of each CTA
             mbar_init(bar(kPpFullV + s), 8u);
             mbar_init(bar(kPpEmptyK + s), 1u);
@@ -517,8 +572,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPpThreads, 1) atten
     const int rows_used = ntok * p.gqa;
     const int row0 = (int)rank * kPpCtaRows;      // first row of this CTA in the tile
     // keys any row of the pair can see (both limits grow with the token)
-    const int kv_lo = row_min_kv(p.batch, g, tok0);
-    const int kv_hi = row_max_kv(p.batch, g, tok0 + ntok - 1);
+    int kv_lo = row_min_kv(p.batch, g, tok0);
+    int kv_hi = row_max_kv(p.batch, g, tok0 + ntok - 1);
+    if (SCORED && (p.sc.key_begin != nullptr || p.sc.key_end != nullptr)) {      // limits of the tokens' own: in no order
+        int lo = 0x7fffffff, hi = -1;
+        for (int t = tok0 + lane; t < tok0 + ntok; t += 32) {
+            if (p.batch.valid_token_mask != nullptr && p.batch.valid_token_mask[g.q_start + t] == 0) continue;
+            const int first = row_first_key<true>(p.batch, p.sc, g, t), last = row_last_key<true>(p.batch, p.sc, g, t);
+            if (first <= last) { lo = min(lo, first); hi = max(hi, last); }
+        }
+        kv_lo = __reduce_min_sync(0xffffffffu, lo);
+        kv_hi = __reduce_max_sync(0xffffffffu, hi);
+    }
     const bool any_keys = kv_hi >= kv_lo;
     const int pg_lo = any_keys ? (kv_lo >> 4) : 0, pg_hi = any_keys ? (kv_hi >> 4) : -1;
     const int all_lo = any_keys ? (kv_lo >> 6) : 0, all = any_keys ? ((kv_hi >> 6) - all_lo + 1) : 0;
@@ -527,7 +592,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPpThreads, 1) atten
 
     __syncwarp();
     if (wid == 0) {
-        tc2_alloc(base + S::kOffBars + 240, 512);
+        tc2_alloc(base + S::kOffBars + S::kWords + 16, 512);
         tc2_relinquish();
     }
     __syncthreads();                 // this CTA's barriers exist
@@ -562,7 +627,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPpThreads, 1) atten
         }
     };
     int32_t next_id = -1;
-    if (wid == 13) {
+    if (!DIRECT && wid == 13) {
         for (int j = 0; j < kPpRawStages && j < nblocks; ++j) {
             const int32_t id = page_id(j);
             copy_k(j, id);
@@ -573,7 +638,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPpThreads, 1) atten
     // The sample that exponents are chosen by: the first scales of the first block's rows, the same in both CTAs.  Requested here,
     // looked at behind the query's rows.
     uint32_t sample_k[2] = {0u, 0u}, sample_v[2] = {0u, 0u};
-    if (wid == 12) {
+    if constexpr (!DIRECT) if (wid == 12) {
         const int32_t id = page_id(0);
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
@@ -617,8 +682,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPpThreads, 1) atten
                     widen8(raw_q[i], p.io_bf16, x);
 #pragma unroll
                     for (int e = 0; e < 8; ++e) x[e] *= p.q_scale;
-                    sts128(q_stage + (uint32_t)row * 512u + (q_chunk_place<ROT>((uint32_t)(j + 8 * i), (uint32_t)row) << 4), pack_half2(x[0], x[1]),
-                           pack_half2(x[2], x[3]), pack_half2(x[4], x[5]), pack_half2(x[6], x[7]));
+                    sts128(q_stage + (uint32_t)row * 512u + (q_chunk_place<ROT>((uint32_t)(j + 8 * i), (uint32_t)row) << 4), pp_pack<FMT>(x[0], x[1]),
+                           pp_pack<FMT>(x[2], x[3]), pp_pack<FMT>(x[4], x[5]), pp_pack<FMT>(x[6], x[7]));
                 }
                 continue;
             }
@@ -657,8 +722,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPpThreads, 1) atten
         }
     }
     if (wid == 12) {
-        const int ek = PpScales<FMT>::exponent(__reduce_max_sync(0xffffffffu, max(sample_k[0], sample_k[1])));
-        const int ev = PpScales<FMT>::exponent(__reduce_max_sync(0xffffffffu, max(sample_v[0], sample_v[1])));
+        int ek = 0, ev = 0;
+        if constexpr (!DIRECT) {
+            ek = PpScales<FMT>::exponent(__reduce_max_sync(0xffffffffu, max(sample_k[0], sample_k[1])));
+            ev = PpScales<FMT>::exponent(__reduce_max_sync(0xffffffffu, max(sample_v[0], sample_v[1])));
+        }
         if (lane == 0) { exponents[0] = ek; exponents[1] = ev; place[0] = req; place[1] = kb_lo; place[2] = tok0; place[3] = rows_used; place[4] = g.q_start; }
     }
     if (ROT) fence_proxy_async();     // the residual tile is read by the tensor core
@@ -694,8 +762,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPpThreads, 1) atten
         // Order in the pipe: QK(0), QK(1), PV(0), QK(2), PV(1), ...  QK(j) overwrites the buffer of P(j - 2),
         // which PV(j - 2), issued before it, has read.
         if (rank == 0 && elect_one()) {
-            constexpr uint32_t kIdescQk = tc_idesc(kPpRows, kPpKeys, 0);
-            constexpr uint32_t kIdescPv = tc_idesc(kPpRows, kHeadDim, 1);
+            constexpr uint32_t kTypes = DIRECT ? (1u << 7) | (1u << 10) : 0u;      // bf16 operands
+            constexpr uint32_t kIdescQk = tc_idesc(kPpRows, kPpKeys, 0) | kTypes;
+            constexpr uint32_t kIdescPv = tc_idesc(kPpRows, kHeadDim, 1) | kTypes;
             const uint64_t desc_k = tc_smem_desc(k_t, 16u, 1024u);
             const uint64_t desc_v = tc_smem_desc(v_t, 4096u, 1024u);
             const uint64_t desc_q = tc_smem_desc(qlo_t, 16u, 1024u);
@@ -710,13 +779,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPpThreads, 1) atten
                         ok = ok && mbar_wait(bar(kPpFullK + (int)kst), kph);
                         if (!ok) break;
                         tc_fence_after();
-                        const uint64_t b0 = desc_k + (uint64_t)(kst * (kPpStage / 16));
+                        const uint64_t b0 = desc_k + (uint64_t)(kst * (S::kStage / 16));
 #pragma unroll
                         for (int ks = 0; ks < 8; ++ks) {
                             const uint64_t b = b0 + (uint64_t)((ks >> 2) * (4096 / 16) + 2 * (ks & 3));
                             const uint32_t a = tmem + kPpColQ + 64u * (uint32_t)h + 8u * (uint32_t)ks;
                             tc2_mma_f16_ts(d, a, b, kIdescQk, (h || ks) ? 1u : 0u);
-                            tc2_mma_f16_ts(d, a, b + kPpPart / 16, kIdescQk, 1u);
+                            if (!DIRECT) tc2_mma_f16_ts(d, a, b + kPpPart / 16, kIdescQk, 1u);
                             if (ROT) {
                                 tc2_mma_f16(d, desc_q + (uint64_t)((2 * h + (ks >> 2)) * (kPpCtaRows * 128 / 16) + 2 * (ks & 3)), b,
                                             kIdescQk, 1u);
@@ -724,7 +793,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPpThreads, 1) atten
                         }
                         tc2_commit_both(bar(kPpEmptyK + (int)kst));
                         if (h == 1) tc2_commit_both(bar(kPpS + (j & 1)));
-                        if (++kst == kPpStages) { kst = 0; kph ^= 1u; }
+                        if (++kst == S::kStages) { kst = 0; kph ^= 1u; }
                     }
                 }
                 if (j > 0 && ok) {
@@ -736,18 +805,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPpThreads, 1) atten
                         ok = ok && mbar_wait(bar(kPpFullV + (int)vst), vph);
                         if (!ok) break;
                         tc_fence_after();
-                        const uint64_t b0 = desc_v + (uint64_t)(vst * (kPpStage / 16));
+                        const uint64_t b0 = desc_v + (uint64_t)(vst * (S::kStage / 16));
 #pragma unroll
                         for (int ks = 0; ks < 2; ++ks) {
                             const uint64_t b = b0 + (uint64_t)((2048 / 16) * ks);
                             const uint32_t a = a0 + 32u * (uint32_t)h + 8u * (uint32_t)ks;
                             tc2_mma_f16_ts(tmem + kPpColO, a, b, kIdescPv, (i > 0 || h > 0 || ks > 0) ? 1u : 0u);
                             tc2_mma_f16_ts(tmem + kPpColO, a + 16u, b, kIdescPv, 1u);
-                            tc2_mma_f16_ts(tmem + kPpColO, a, b + kPpPart / 16, kIdescPv, 1u);
+                            if (!DIRECT) tc2_mma_f16_ts(tmem + kPpColO, a, b + kPpPart / 16, kIdescPv, 1u);
                         }
                         tc2_commit_both(bar(kPpEmptyV + (int)vst));
                         if (h == 1) tc2_commit_both(bar(kPpPv + (i & 1)));
-                        if (++vst == kPpStages) { vst = 0; vph ^= 1u; }
+                        if (++vst == S::kStages) { vst = 0; vph ^= 1u; }
                     }
                 }
             }
@@ -758,6 +827,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPpThreads, 1) atten
         __syncwarp();
         if (!wait_all(bar(kPpDrain), 0u)) *abort_flag = 1u;
     } else if (wid == 13) {
+        if constexpr (!DIRECT) {
         // ======================= copy issue: raw (page, head) runs of a block ===========================
         int issued = 2 * min(nblocks, kPpRawStages);
 #pragma unroll 1
@@ -777,7 +847,66 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPpThreads, 1) atten
         const int kn = (issued + 1) / 2, vn = issued / 2;
         for (int j = max(0, kn - kPpRawStages); j < kn; ++j) (void)wait_all(bar(kPpRawKFull + j % kPpRawStages), (uint32_t)((j / kPpRawStages) & 1));
         for (int j = max(0, vn - kPpRawStages); j < vn; ++j) (void)wait_all(bar(kPpRawVFull + j % kPpRawStages), (uint32_t)((j / kPpRawStages) & 1));
+        }
+    } else if (DIRECT && wid >= 4) {
+        if constexpr (DIRECT) {
+        // ======================= BF16 rows straight into the tiles: lane = key, this warp's 32 channels of the stage's 128 ========
+        const bool is_v = wid >= 8;
+        const int quarter = wid & 3;
+        const int full = is_v ? kPpFullV : kPpFullK, empty = is_v ? kPpEmptyV : kPpEmptyK;
+        const uint8_t* head = is_v ? v_head_base : k_head_base;
+        const uint64_t page_stride = is_v ? p.layout.v_page_stride_bytes : p.layout.k_page_stride_bytes;
+        const uint64_t token_stride = is_v ? p.layout.v_token_stride_bytes : p.layout.k_token_stride_bytes;
+        const uint32_t tile0 = (is_v ? v_t : k_t) + (uint32_t)(quarter >> 1) * 4096u + (uint32_t)lane * 128u;
+        const uint32_t leader_full = map_to_rank(bar(full), 0u);
+        // Key of this lane in half h of block j; K: the CTA's 32 keys in both halves.  Pages are looked up a block ahead.
+        auto key_of = [&](int j, int h) { return ((kb_lo + j) << 6) + 32 * (is_v ? h : (int)rank) + lane; };
+        auto page_of = [&](int j, int h) -> int32_t {
+            const int pos = key_of(j, h);
+            return j < nblocks && pos >= kv_lo && pos <= kv_hi ? block_table_page(blocks, pos >> 4, p.batch.max_blocks_per_req, kInBf16) : -1;
+        };
+        int32_t page[2] = {page_of(0, 0), page_of(0, 1)};
+        constexpr int kAhead = S::kStages - 2;      // copies in flight
+        int issued = 0, told = 0;
+        auto tell = [&]() {      // the oldest stage that is not known to the MMA warp: this thread's copies into it have landed
+            fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cluster(leader_full + 8u * (uint32_t)(told % S::kStages));
+            ++told;
+        };
+#pragma unroll 1
+        for (int j = 0; j < nblocks; ++j) {
+            if (aborted_any()) break;
+            const int32_t next[2] = {page_of(j + 1, 0), page_of(j + 1, 1)};
+            bool ok = true;
+#pragma unroll 1
+            for (int h = 0; h < 2; ++h) {
+                const int st = issued % S::kStages;
+                // parity 1: the first pass over the ring does not wait
+                ok = wait_all(bar(empty + st), (uint32_t)((issued / S::kStages + 1) & 1));
+                if (!ok) break;
+                const int32_t id = page[h];
+                const uint8_t* src = head + (id < 0 ? 0 : (size_t)id * page_stride + (size_t)(key_of(j, h) & 15) * token_stride) +
+                                     256 * (is_v ? (int)rank : h) + 64 * quarter;
+                const uint32_t dst = tile0 + (uint32_t)st * S::kStage;
+#pragma unroll
+                for (int c = 0; c < 4; ++c) pp_copy16(dst + (uint32_t)(((4 * (quarter & 1) + c) ^ (lane & 7)) << 4), src + 16 * c, id >= 0);
+                asm volatile("cp.async.commit_group;" ::: "memory");
+                ++issued;
+                if (issued > kAhead) {
+                    asm volatile("cp.async.wait_group %0;" ::"n"(kAhead) : "memory");
+                    tell();
+                }
+            }
+            if (!ok) { *abort_flag = 1u; break; }
+            page[0] = next[0];
+            page[1] = next[1];
+        }
+        asm volatile("cp.async.wait_group 0;" ::: "memory");      // (after an abort as well: nothing is in flight when the CTA leaves)
+        while (told < issued) tell();
+        }
     } else if (wid >= 4) {
+        if constexpr (!DIRECT) {
         // ======================= producers: lane = key, this warp's 32 channels of the stage's 128 ========
         const bool is_v = wid >= 8;
         const int quarter = wid & 3;
@@ -904,14 +1033,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPpThreads, 1) atten
                 }
             }
         }
+        }
     } else {
         // ======================= consumers: softmax, P, rescale =========================================
         const int trow = row0 + tid;
         const int q_off = tok0 + trow / p.gqa;
         const bool row_ok = trow < rows_used &&
                             (p.batch.valid_token_mask == nullptr || p.batch.valid_token_mask[g.q_start + q_off] != 0);
-        const int rmax = row_ok ? row_max_kv(p.batch, g, q_off) : -1;
-        const int rmin = row_ok ? row_min_kv(p.batch, g, q_off) : 0x7fffffff;
+        const int rmax = row_ok ? row_last_key<SCORED>(p.batch, p.sc, g, q_off) : -1;
+        const int rmin = row_ok ? row_first_key<SCORED>(p.batch, p.sc, g, q_off) : 0x7fffffff;
+        const float slope = SCORED && row_ok ? row_slope(p.sc, kv_head * p.gqa + trow % p.gqa) : 0.0f;
         const uint32_t lane_base = (uint32_t)(32 * wid) << 16;
         const uint32_t t_o = tmem + lane_base + kPpColO, t_s = tmem + lane_base + kPpColS;
         const uint32_t leader_pready = map_to_rank(bar(kPpPReady), 0u);
@@ -931,7 +1062,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPpThreads, 1) atten
             // Scores of keys [32 c, + 32) of the block, masked.  TQ4: `factor`, the exponent's power of two, is still to be applied.  8-bit:
             // p.score_scale is, a constant operand (in one register with the power of two it made these builds spill, and a stack
             // frame costs this kernel several us a launch).
-            auto scores = [&](int c, float (&sv)[32]) {
+            // SCORED: they are changed here, `factor` or p.score_scale first (TQ4: and put back for the second read).
+            auto scores = [&](int c, float (&sv)[32], bool again = false) {
                 uint32_t r[32];
                 tc_ld32(r, t_sj + 32u * (uint32_t)c);
                 tc_wait_ld();
@@ -942,12 +1074,23 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPpThreads, 1) atten
 #pragma unroll
                     for (int i = 0; i < 32; ++i) sv[i] *= up;
                 }
-                if (!all_seen) {
+                if (SCORED && !again) {
+                    const float away = (float)(g.ctx_before + q_off - (kbase + 32 * c));
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) sv[i] = changed_score(p.sc, sv[i] * (ROT ? factor : p.score_scale), slope, away - (float)i);
+                }
+                if (!all_seen && !(SCORED && again)) {
 #pragma unroll
                     for (int i = 0; i < 32; ++i) {
                         const int pos = kbase + 32 * c + i;
                         if (!(pos >= rmin && pos <= rmax)) sv[i] = -INFINITY;
                     }
+                }
+                if (SCORED && ROT && !again) {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(sv[i]);
+                    tc_st32(t_sj + 32u * (uint32_t)c, r);
+                    tc_wait_st();
                 }
             };
             // TQ4 reads them twice (maximum, then weights): holding all 64 spills there (92 bytes a thread, five ragged
@@ -960,7 +1103,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPpThreads, 1) atten
 #pragma unroll
                 for (int i = 0; i < 32; ++i) mx4[i & 3] = fmaxf(mx4[i & 3], sv[ROT ? 0 : c][i]);
             }
-            const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * (ROT ? factor : p.score_scale);
+            const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * (SCORED ? 1.0f : ROT ? factor : p.score_scale);
             // the reference maximum moves only when the true maximum ran ahead by more than the threshold
             const bool need = mx > m_ref + kPpRescaleThreshold;
             float alpha = 1.0f;
@@ -987,17 +1130,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPpThreads, 1) atten
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
                 uint32_t hi[16], lo[16];
-                if (ROT) scores(c, sv[0]);
+                if (ROT) scores(c, sv[0], true);
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
                     // masked scores are -infinity: ex2 gives exactly 0 against any finite reference
                     const float sa = sv[ROT ? 0 : c][2 * i], sb = sv[ROT ? 0 : c][2 * i + 1];
-                    const float pa = ex2(__fmaf_rn(sa, ROT ? factor : p.score_scale, -m_use)), pb = ex2(__fmaf_rn(sb, ROT ? factor : p.score_scale, -m_use));
+                    const float pa = SCORED ? ex2(sa - m_use) : ex2(__fmaf_rn(sa, ROT ? factor : p.score_scale, -m_use));
+                    const float pb = SCORED ? ex2(sb - m_use) : ex2(__fmaf_rn(sb, ROT ? factor : p.score_scale, -m_use));
                     ls4[i & 3] += pa + pb;
-                    const __half2 h = __floats2half2_rn(pa, pb);
-                    const float2 hf = __half22float2(h);
-                    hi[i] = *reinterpret_cast<const uint32_t*>(&h);
-                    lo[i] = pack_half2(pa - hf.x, pb - hf.y);
+                    hi[i] = pp_pack<FMT>(pa, pb);
+                    const float2 hf = pp_unpack<FMT>(hi[i]);
+                    lo[i] = pp_pack<FMT>(pa - hf.x, pb - hf.y);
                 }
                 // P takes the place of the scores it came from: value in columns 32 c .. + 15, residual in the next 16
                 tc_st16(t_sj + 32u * c, hi);
@@ -1024,7 +1167,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPpThreads, 1) atten
     bool fits = true;
     if ((k_exp | v_exp) != 0) {      // does every row of the tile fit the sample's exponents?  (K rows are spread over both CTAs.)
         cluster_sync_all();
-        fits = PpScales<FMT>::fits(row_max[0], k_exp) && PpScales<FMT>::fits(row_max[1], v_exp);
+        if constexpr (!DIRECT) fits = PpScales<FMT>::fits(row_max[0], k_exp) && PpScales<FMT>::fits(row_max[1], v_exp);
     }
     const bool aborted = *abort_flag != 0u;
     float* stage = reinterpret_cast<float*>(gen);
@@ -1062,8 +1205,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPpThreads, 1) atten
                 float l = src[256], m = src[257];
                 float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
                 if (!fits) {
-                    prefill_row_fp32<FMT>(p, place[0], q_off, q_head, place[1] << 6, ((place[1] + nblocks) << 6) - 1, v, l, m);
-                } else if (PpFormat<FMT>::has_keys(l)) {
+                    if constexpr (SCORED) {      // (the mass and rows of the other splits carry 2^kPpShift)
+                        const ScoredRow one = {&p.layout, &p.batch, &p.sc, p.q_in, p.io_bf16, p.num_q_heads, p.gqa};
+                        scored_row_keys(one, place[0], q_off, q_head, place[1] << 6, ((place[1] + nblocks) << 6) - 1, 0, 1, v, m, l);
+                        const float up = (float)(1 << (int)kPpShift);
+                        l *= up;
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) v[i] *= ROT ? up * kPpLutScale : up;
+                    } else if constexpr (!DIRECT) {
+                        prefill_row_fp32<FMT>(p, place[0], q_off, q_head, place[1] << 6, ((place[1] + nblocks) << 6) - 1, v, l, m);
+                    }
+                } else if (SCORED ? l != 0.0f : PpFormat<FMT>::has_keys(l)) {
                     const uint32_t qa = ROT ? quad_place(2u * lane) : 2u * lane;      // (the next quad is its neighbour)
                     const float4 a = *reinterpret_cast<const float4*>(src + 4u * qa), b = *reinterpret_cast<const float4*>(src + 4u * (qa ^ 1u));
                     v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
@@ -1082,7 +1234,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPpThreads, 1) atten
                     if (lane == 0) p.parts_ml[part_row] = make_float2(m, l);
                     continue;
                 }
-                prefill_finish_row<ROT>(p, v, l, out_row * kHeadDim, lane);
+                if constexpr (SCORED) prefill_finish_scored_row<ROT>(p, v, l, place[0], q_off, q_head, lane);
+                else prefill_finish_row<ROT>(p, v, l, out_row * kHeadDim, lane);
             }
         } else {
             const int r4 = lane >> 3, j = lane & 7;
@@ -1097,7 +1250,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPpThreads, 1) atten
                 const uint32_t at = smem_u32(smem_raw) + (uint32_t)row * (4u * kPpOutStride);
                 const float l = __uint_as_float(lds32(at + 1024u));
                 float inv = l > 0.0f ? 1.0f / (ROT ? l * (kPpLutScale * 16.0f) : l) : 0.0f;
-                const bool keys = PpFormat<FMT>::has_keys(l);
+                const bool keys = SCORED ? l != 0.0f : PpFormat<FMT>::has_keys(l);
                 if (v_exp != 0) inv *= power_of_two(v_exp);
                 float v[32];
                 const auto chunk_quad = [&](int k) { return (uint32_t)(2 * (j + 8 * (k >> 1)) + (k & 1)); };
@@ -1121,6 +1274,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPpThreads, 1) atten
                 }
                 if (ROT) rotate_registers<4 + 8 + 16>(v);
                 const uint32_t signs = ROT ? chunk_signs(j) : 0u;
+                uint32_t again = 0u;      // SCORED: lanes of rows that are not finite
+                if (SCORED) {
+                    bool fine = is_finite(l);
+#pragma unroll
+                    for (int k = 0; k < 32; ++k) fine = fine && is_finite(v[k]);
+                    again = __ballot_sync(0xffffffffu, ok && !fine);
+                }
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     float x[8];
@@ -1129,6 +1289,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPpThreads, 1) atten
                     apply_output_gate8(x, p.og, gate[i & 1], lane, p.io_bf16);
                     if (i < 2 && gated) load8_raw(p.og.gate, out_base, j + 8 * (i + 2), gate[i & 1]);
                     if (ok) store8(p.attn_out, out_base, j + 8 * i, p.io_bf16, x);
+                }
+                if (SCORED && again != 0u) {
+                    __syncwarp();      // the rows that follow overwrite what was just stored
+#pragma unroll 1
+                    for (int q = 0; q < 4; ++q) {
+                        if (((again >> (8 * q)) & 0xffu) == 0u) continue;
+                        const int r = (int)cluster_rank() * kPpCtaRows + 4 * grp + q;
+                        const int off = first_token + r / p.gqa, head = kv_head * p.gqa + r % p.gqa;
+                        const ScoredRow one = {&p.layout, &p.batch, &p.sc, p.q_in, p.io_bf16, p.num_q_heads, p.gqa};
+                        float y[8];
+                        scored_row_whole(one, place[0], off, head, y);
+                        store8(p.attn_out, ((size_t)(q_start + off) * p.num_q_heads + head) * kHeadDim, lane, p.io_bf16, y);
+                    }
                 }
             }
         }
@@ -1200,9 +1373,10 @@ static PrefillPairPlan prefill_pair_plan(const warp34_exec* ex, const warp34_kv_
 }
 
 // The pair kernel for one layer's chunk.  Workspace: a status word, and room for the parts when it splits.
-template <int FMT>
+template <int FMT, bool SCORED = false>
 static int launch_prefill_pair(const warp34_exec* ex, const warp34_kv_layer_layout* layout, const warp34_attention_batch* batch,
-                               const void* q_in, void* attn_out, int num_q_heads, int io_bf16, const OutputGate& og, int sm_count, int skip_rows = 0) {
+                               const void* q_in, void* attn_out, int num_q_heads, int io_bf16, const OutputGate& og, int sm_count, int skip_rows = 0,
+                               const ScoreChange& sc = ScoreChange()) {
     int32_t* status = nullptr;      // the first word of the workspace, when there is one
     if (ex->scratch_ptr != 0 && (ex->scratch_ptr & 3u) == 0 && ex->scratch_size >= sizeof(PlanHeader)) {
         status = reinterpret_cast<int32_t*>((uintptr_t)ex->scratch_ptr);   // PlanHeader::status
@@ -1227,6 +1401,7 @@ static int launch_prefill_pair(const warp34_exec* ex, const warp34_kv_layer_layo
     }
     pp.status = status;
     pp.og = og;
+    pp.sc = sc;
     pp.skip_tokens = skip_rows / pp.gqa;
     const PrefillPairPlan plan = prefill_pair_plan(ex, layout, batch, num_q_heads, sm_count, skip_rows);
     const long long tiles = plan.tiles;
@@ -1242,9 +1417,9 @@ static int launch_prefill_pair(const warp34_exec* ex, const warp34_kv_layer_layo
     }
     cudaStream_t st = (cudaStream_t)ex->stream;
     const dim3 grid(2u * (unsigned)tiles, (unsigned)layout->local_kv_heads, (unsigned)pp.splits);
-    int rc = launch_behind(attention_prefill_pair_kernel<FMT>, grid, kPpThreads, PpSmem<FMT>::kBytes, st, pp);
+    int rc = launch_behind(attention_prefill_pair_kernel<FMT, SCORED>, grid, kPpThreads, PpSmem<FMT>::kBytes, st, pp);
     if (rc == 0 && pp.splits > 1) {
-        rc = launch_behind(prefill_merge_kernel<PpFormat<FMT>::kRotated>, dim3((unsigned)((rows + 3) / 4)), 128, 0, st, pp);
+        rc = launch_behind(prefill_merge_kernel<PpFormat<FMT>::kRotated, SCORED>, dim3((unsigned)((rows + 3) / 4)), 128, 0, st, pp);
     }
     return rc;
 }

@@ -1,0 +1,53 @@
+// What warp34_paged_attention_scored_* changes between the product of a query with a key and the softmax, shared by the attention kernels:
+//
+//   t = sm_scale q k;   t <- cap tanh(t / cap);   t <- t - slope[head] |position of the query - position of the key|
+//   key visible iff  first(token) <= position <= last(token)
+//
+// Kernels hold scores in units of log2(e) (weights are powers of two), so the factors here are as well.
+// tanh(x) = 1 - 2 / (e^(2 x) + 1), two special-function instructions: 1.5 x 2^-23 of the cap off at most (sum and reciprocal), which is
+// 2e-4 of a weight at the largest cap that is accepted.  (tanh.approx, one instruction, is off by 2^-11 of the cap: 2.5 % of a weight
+// at a cap of 50.)
+// Included by tq4_attention.cu.
+#pragma once
+
+namespace w34 {
+
+constexpr float kMaxSoftcap = 1024.0f, kMinSoftcap = 1.0f / 1024.0f;
+
+struct ScoreChange {
+    float cap = 0.0f;         // x log2(e); 0: scores are not capped
+    float cap_arg = 0.0f;     // 2 / cap: what makes a score the exponent of e^(2 t / cap)
+    const float* slopes = nullptr;           // [q heads]
+    const int32_t* key_begin = nullptr;      // [tokens] first key, or null
+    const int32_t* key_end = nullptr;        // [tokens] key behind the last, in place of causality, or null
+};
+
+// First and last key of a row.  SCORED: the token's own limits as well.
+template <bool SCORED>
+__device__ __forceinline__ int row_first_key(const warp34_attention_batch& b, const ScoreChange& sc, const ReqGeom& g, int q_off) {
+    int m = row_min_kv(b, g, q_off);
+    if (SCORED && sc.key_begin != nullptr) m = max(m, sc.key_begin[g.q_start + q_off]);
+    return m;
+}
+template <bool SCORED>
+__device__ __forceinline__ int row_last_key(const warp34_attention_batch& b, const ScoreChange& sc, const ReqGeom& g, int q_off) {
+    if (SCORED && sc.key_end != nullptr) return min(max(sc.key_end[g.q_start + q_off], 0), g.seq_after) - 1;
+    return row_max_kv(b, g, q_off);
+}
+
+// The change of one score: `slope` in log2(e) units (0: none), `away` position of the query less that of the key.  (Callers make it from one
+// conversion for a row and a block of keys, and subtract the key's place there: int to float is as dear as a reciprocal.)
+__device__ __forceinline__ float changed_score(const ScoreChange& sc, float t, float slope, float away) {
+    if (sc.cap != 0.0f) {      // uniform
+        float e, r;
+        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(t * sc.cap_arg));
+        asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(e + 1.0f));
+        t = __fmaf_rn(-2.0f * sc.cap, r, sc.cap);
+    }
+    return __fmaf_rn(-slope, fabsf(away), t);
+}
+__device__ __forceinline__ float row_slope(const ScoreChange& sc, int q_head) { return sc.slopes != nullptr ? sc.slopes[q_head] * 1.4426950408889634f : 0.0f; }
+
+__device__ __forceinline__ bool is_finite(float x) { return fabsf(x) <= 3.402823466e38f; }
+
+}  // namespace w34

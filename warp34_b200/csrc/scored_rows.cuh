@@ -1,0 +1,191 @@
+// Attention with changed scores, a row at a time in fp32, over every layer format and any strides: the kernel for calls that the
+// tensor-core kernels do not take (no workspace, other packings, mixed 8-bit formats, WARP34_B200_EXEC_FLAG_PRECISE_ATTENTION), and the
+// second look at rows that came out non-finite.  The latter because a product of a tile's weights with its V rows meets every row of
+// the tile with every key of it: a NaN or infinity in the V of a key that one row must not see (another document's, say) is 0 x NaN there.
+// A row that has such a key in sight comes out non-finite again.
+// Included by tq4_attention.cu.
+#pragma once
+
+namespace w34 {
+
+// Columns [8 lane, + 8) of a stored row (TQ4: in the rotated basis).
+__device__ __forceinline__ void scored_elements(const uint8_t* row, int format, int lane, float (&x)[8]) {
+    if (format == WARP34_KV_FORMAT_TQ4) {
+        const uint8_t* half = row + kTq4BlockBytes * (lane >> 4);
+        const uint16_t* codes = reinterpret_cast<const uint16_t*>(half + 2 + 4 * (lane & 15));
+        const float d = __half2float(*reinterpret_cast<const __half*>(half));
+        const uint32_t w = (uint32_t)codes[0] | ((uint32_t)codes[1] << 16);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = d * tq4_centroid((int)((w >> (4 * i)) & 15u));
+    } else if (format == WARP34_KV_FORMAT_BF16) {
+        const uint16_t* src = reinterpret_cast<const uint16_t*>(row) + 8 * lane;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = __uint_as_float((uint32_t)src[i] << 16);
+    } else {
+        const bool fp8 = format == WARP34_KV_FORMAT_FP8_E4M3;
+        const uint32_t* codes = reinterpret_cast<const uint32_t*>(row + (fp8 ? 8 * lane : 68 * (lane >> 3) + 4 + 8 * (lane & 7)));
+        const float d = *reinterpret_cast<const float*>(row + (fp8 ? kHeadDim + 4 * (lane >> 4) : 68 * (lane >> 3)));
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            uint32_t a, b;
+            if (fp8) kv8x4_to_f16x4<WARP34_KV_FORMAT_FP8_E4M3>(codes[i], a, b);
+            else kv8x4_to_f16x4<WARP34_KV_FORMAT_Q8_0>(codes[i], a, b);
+            const float2 fa = __half22float2(*reinterpret_cast<const __half2*>(&a)), fb = __half22float2(*reinterpret_cast<const __half2*>(&b));
+            x[4 * i] = d * fa.x; x[4 * i + 1] = d * fa.y; x[4 * i + 2] = d * fb.x; x[4 * i + 3] = d * fb.y;
+        }
+    }
+}
+
+struct ScoredRow {
+    const warp34_kv_layer_layout* layout;
+    const warp34_attention_batch* batch;
+    const ScoreChange* sc;
+    const void* q_in;
+    int io_bf16, num_q_heads, gqa;
+};
+
+// Keys first, first + step, ... of [lo, hi] of one query row by one warp: columns [8 lane, + 8) of sum w V (stored basis), running
+// maximum (log2 units) and mass.
+__device__ __forceinline__ void scored_row_keys(const ScoredRow& p, int req, int q_off, int q_head, int lo, int hi, int first, int step, float (&acc)[8],
+                                             float& m, float& l) {
+    const int lane = threadIdx.x & 31, kv_head = q_head / p.gqa;
+    const warp34_attention_batch& b = *p.batch;
+    const warp34_kv_layer_layout& lay = *p.layout;
+    const ReqGeom g = load_req(b, req);
+    const int32_t* blocks = b.block_tables + (size_t)req * b.max_blocks_per_req;
+    const uint8_t* k_head = (const uint8_t*)(uintptr_t)lay.k_base + (size_t)kv_head * lay.k_head_stride_bytes;
+    const uint8_t* v_head = (const uint8_t*)(uintptr_t)lay.v_base + (size_t)kv_head * lay.v_head_stride_bytes;
+    lo = max(lo, row_first_key<true>(b, *p.sc, g, q_off));
+    hi = min(hi, row_last_key<true>(b, *p.sc, g, q_off));
+    float q[8];
+    load8(p.q_in, ((size_t)(g.q_start + q_off) * p.num_q_heads + q_head) * kHeadDim, lane, p.io_bf16, q);
+    float scale = b.sm_scale * 1.4426950408889634f;
+    if (lay.k_format == WARP34_KV_FORMAT_TQ4) {
+        sign8(q, lane);
+        butterfly8<5>(q, lane);
+        scale *= 0.0625f;
+    }
+    const float slope = row_slope(*p.sc, q_head);
+    const int q_pos = g.ctx_before + q_off;
+    m = -1e30f;
+    l = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) acc[i] = 0.0f;
+    if (lo > hi) return;
+#pragma unroll 1
+    for (int pos0 = lo + first; pos0 <= hi; pos0 += 2 * step) {
+        const uint8_t* vrow[2];
+        float s[2];
+        bool use[2];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {      // two keys at a time, so that two rows are on their way
+            use[k] = pos0 + k * step <= hi;
+            const int pos = use[k] ? pos0 + k * step : pos0;
+            const int page = block_table_page(blocks, pos >> 4, b.max_blocks_per_req, kInScalar);
+            const size_t off = pos & 15;
+            float x[8];
+            scored_elements(k_head + (size_t)page * lay.k_page_stride_bytes + off * lay.k_token_stride_bytes, lay.k_format, lane, x);
+            vrow[k] = v_head + (size_t)page * lay.v_page_stride_bytes + off * lay.v_token_stride_bytes;
+            float d = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) d = __fmaf_rn(q[i], x[i], d);
+            s[k] = changed_score(*p.sc, warp_sum(d) * scale, slope, (float)(q_pos - pos));
+        }
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            if (!use[k]) continue;
+            const float m_new = fmaxf(m, s[k]), alpha = ex2(m - m_new), w = ex2(s[k] - m_new);
+            float x[8];
+            scored_elements(vrow[k], lay.v_format, lane, x);
+            l = l * alpha + w;
+            m = m_new;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) acc[i] = __fmaf_rn(acc[i], alpha, w * x[i]);
+        }
+    }
+}
+
+// The same for all of a row's keys, normalised and in the natural basis.
+__device__ __forceinline__ void scored_row_whole(const ScoredRow& p, int req, int q_off, int q_head, float (&v)[8]) {
+    float m, l;
+    scored_row_keys(p, req, q_off, q_head, 0, 0x7ffffffe, 0, 1, v, m, l);
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    const bool rotated = p.layout->v_format == WARP34_KV_FORMAT_TQ4;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] *= rotated ? inv * 0.0625f : inv;
+    if (rotated) {
+        butterfly8<5>(v, threadIdx.x & 31);
+        sign8(v, threadIdx.x & 31);
+    }
+}
+
+// One block of four warps per (token, q head); warp w takes the keys first + w, + 4, ...
+struct ScoredParams {
+    warp34_kv_layer_layout layout;
+    warp34_attention_batch batch;
+    ScoreChange sc;
+    const void* q_in;
+    void* attn_out;
+    int io_bf16, num_q_heads;
+};
+__global__ void __launch_bounds__(128) scored_rows_kernel(const __grid_constant__ ScoredParams p) {
+    __shared__ __align__(16) float s_acc[4][kHeadDim];
+    __shared__ float s_m[4], s_l[4];
+    grid_dependency_wait();
+    grid_launch_dependents();
+    const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
+    const int tok = (int)(blockIdx.x / (unsigned)p.num_q_heads), q_head = (int)(blockIdx.x % (unsigned)p.num_q_heads);
+    if (p.batch.valid_token_mask != nullptr && p.batch.valid_token_mask[tok] == 0) return;   // block-uniform exits
+    const int req = find_request(p.batch.query_start_loc, p.batch.num_reqs, tok);
+    if (req < 0 || !load_req(p.batch, req).valid) return;
+    const ScoredRow row = {&p.layout, &p.batch, &p.sc, p.q_in, p.io_bf16, p.num_q_heads, p.num_q_heads / p.layout.local_kv_heads};
+    float acc[8], m, l;
+    scored_row_keys(row, req, tok - p.batch.query_start_loc[req], q_head, 0, 0x7ffffffe, wid, 4, acc, m, l);
+    *reinterpret_cast<float4*>(&s_acc[wid][8 * lane]) = make_float4(acc[0], acc[1], acc[2], acc[3]);
+    *reinterpret_cast<float4*>(&s_acc[wid][8 * lane + 4]) = make_float4(acc[4], acc[5], acc[6], acc[7]);
+    if (lane == 0) { s_m[wid] = m; s_l[wid] = l; }
+    __syncthreads();
+    if (wid != 0) return;
+    const float m_tot = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3]));
+    float l_tot = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) acc[i] = 0.0f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        if (s_l[w] == 0.0f) continue;      // no keys
+        const float wgt = ex2(s_m[w] - m_tot);
+        l_tot += s_l[w] * wgt;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) acc[i] += s_acc[w][8 * lane + i] * wgt;
+    }
+    const bool rotated = p.layout.v_format == WARP34_KV_FORMAT_TQ4;
+    const float inv = l_tot == 0.0f ? 0.0f : 1.0f / l_tot;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) acc[i] *= rotated ? inv * 0.0625f : inv;
+    if (rotated) {
+        butterfly8<5>(acc, lane);
+        sign8(acc, lane);
+    }
+    store8(p.attn_out, ((size_t)tok * p.num_q_heads + q_head) * kHeadDim, lane, p.io_bf16, acc);
+}
+
+static int launch_scored_rows(const warp34_exec* ex, const warp34_kv_layer_layout* layout, const warp34_attention_batch* batch, const ScoreChange& sc,
+                              const void* q_in, void* attn_out, int num_q_heads, int io_bf16) {
+    const uint64_t bits = layout->k_base | layout->v_base | layout->k_page_stride_bytes | layout->k_head_stride_bytes | layout->k_token_stride_bytes |
+                          layout->v_page_stride_bytes | layout->v_head_stride_bytes | layout->v_token_stride_bytes;
+    const bool words = layout->k_format == WARP34_KV_FORMAT_Q8_0 || layout->k_format == WARP34_KV_FORMAT_FP8_E4M3;
+    if ((bits & (words ? 3u : 1u)) != 0u) return (int)cudaErrorInvalidValue;
+    const long long rows = (long long)batch->total_tokens * num_q_heads;
+    if (rows > 0x7fffffffll) return (int)cudaErrorInvalidValue;
+    ScoredParams p;
+    p.layout = *layout;
+    p.batch = *batch;
+    p.sc = sc;
+    p.q_in = q_in;
+    p.attn_out = attn_out;
+    p.io_bf16 = io_bf16;
+    p.num_q_heads = num_q_heads;
+    return launch_behind(scored_rows_kernel, dim3((unsigned)rows), 128, 0, (cudaStream_t)ex->stream, p);
+}
+
+}  // namespace w34

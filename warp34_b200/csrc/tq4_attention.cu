@@ -68,6 +68,10 @@ __device__ __forceinline__ int row_min_kv(const warp34_attention_batch& b, const
     return m;
 }
 
+}  // namespace w34
+#include "score_change.cuh"
+namespace w34 {
+
 // Activations are fp16 (the reference ABI) or bf16 (additive entry points): 16-bit loads and
 // stores with the conversion picked at run time, outside the per-page loops.
 __device__ __forceinline__ float load_act(const void* base, size_t idx, int bf16) {
@@ -591,6 +595,7 @@ struct StreamParams {
     const int32_t* num_selected = nullptr;
     const int32_t* seq_pos = nullptr;
     int select_k = 0;
+    ScoreChange sc = {};   // SCORED builds and the plan in front of them
 };
 
 // Geometry of request r: from the batch descriptor, or in query-sparse mode one query token at
@@ -660,8 +665,19 @@ __global__ void __launch_bounds__(kPlanThreads) tq4_attention_plan_kernel(const 
         } else if (r < R) {
             const ReqGeom g = load_req(p.batch, r);
             if (g.valid && (p.max_rows == 0 || g.q_len <= p.max_rows / p.gqa)) {
-                const int lo = row_min_kv(p.batch, g, 0);
-                const int hi = row_max_kv(p.batch, g, g.q_len - 1);
+                int lo = row_min_kv(p.batch, g, 0);
+                int hi = row_max_kv(p.batch, g, g.q_len - 1);
+                if (p.sc.key_begin != nullptr || p.sc.key_end != nullptr) {      // limits of the tokens' own: in no order
+                    lo = 0x7fffffff;
+                    hi = -1;
+                    for (int t = 0; t < g.q_len; ++t) {
+                        if (p.batch.valid_token_mask != nullptr && p.batch.valid_token_mask[g.q_start + t] == 0) continue;
+                        const int first = row_first_key<true>(p.batch, p.sc, g, t), last = row_last_key<true>(p.batch, p.sc, g, t);
+                        if (first > last) continue;
+                        lo = min(lo, first);
+                        hi = max(hi, last);
+                    }
+                }
                 if (hi >= lo) { plo = lo >> 4; npages = (hi >> 4) - plo + 1; }
                 ngroups = (g.q_len * p.gqa + p.rows_per_group - 1) / p.rows_per_group;
                 // a request longer than the batch's max_q_len has no room in the fragment store
@@ -1375,6 +1391,7 @@ __device__ __forceinline__ void sts128(uint32_t addr, uint32_t a, uint32_t b, ui
 W34_BOUNDS_HOST_HOOKS(attention)
 
 }  // namespace w34
+#include "scored_rows.cuh"
 #include "tq4_stream_exact.cuh"
 #include "tq4_prefill_tc.cuh"
 #include "prefill_pair.cuh"
@@ -1391,8 +1408,9 @@ constexpr int kRowTripleFloats = kHeadDim + 2;
 // either normalise + inverse rotation + fp16 store, or (PARTIAL_OUT) store the merged
 // (acc, m, l) triple for a cross-shard merge.  MW = 4 for batches; a long single sequence has
 // hundreds of partials per row and only a few rows, for which MW = 32.
-template <bool PARTIAL_OUT, int MW>
-__global__ void __launch_bounds__(MW * 32) tq4_attention_merge_kernel(const StreamParams p) {
+// SCORED: a state that is not finite is kept, and a row that ends so is computed again by itself (scored_rows.cuh).
+template <bool PARTIAL_OUT, int MW, bool SCORED = false>
+__global__ void __launch_bounds__(MW * 32) tq4_attention_merge_kernel(const __grid_constant__ StreamParams p) {
     __shared__ __align__(16) float s_acc[MW][kHeadDim];
     __shared__ float s_m[MW], s_l[MW];
     grid_dependency_wait();
@@ -1452,6 +1470,7 @@ __global__ void __launch_bounds__(MW * 32) tq4_attention_merge_kernel(const Stre
     float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};      // columns [8 lane, + 8)
     float l_tot = 0.0f;
     float m_tot = -1e30f;
+    bool odd = false;      // SCORED: a part's mass is not finite
     if (npages > 0 && per > 0) {
         const int us = unit_prefix[r] + item * npages;
         const int w_first = us / per, w_last = (us + npages - 1) / per;
@@ -1468,6 +1487,7 @@ __global__ void __launch_bounds__(MW * 32) tq4_attention_merge_kernel(const Stre
                 const float* ps = base + (size_t)mine * part_floats + rpg * kHeadDim;
                 l_s = ps[rpg + row8];
                 m_s = ps[row8];
+                if (SCORED) odd = odd || !is_finite(l_s);
                 if (!(l_s > 0.0f)) { l_s = 0.0f; m_s = -1e30f; }
             }
             float m_chunk = m_s;
@@ -1509,7 +1529,8 @@ __global__ void __launch_bounds__(MW * 32) tq4_attention_merge_kernel(const Stre
     // combine the warps
     *reinterpret_cast<float4*>(&s_acc[wid][8 * lane]) = make_float4(acc[0], acc[1], acc[2], acc[3]);
     *reinterpret_cast<float4*>(&s_acc[wid][8 * lane + 4]) = make_float4(acc[4], acc[5], acc[6], acc[7]);
-    if (lane == 0) { s_m[wid] = m_tot; s_l[wid] = l_tot; }
+    if (SCORED) odd = __any_sync(0xffffffffu, odd);
+    if (lane == 0) { s_m[wid] = m_tot; s_l[wid] = SCORED && odd ? __uint_as_float(0x7fc00000u) : l_tot; }
     __syncthreads();
     if (wid != 0) return;
     m_tot = s_m[0];
@@ -1521,7 +1542,7 @@ __global__ void __launch_bounds__(MW * 32) tq4_attention_merge_kernel(const Stre
 #pragma unroll 4
     for (int w = 0; w < MW; ++w) {
         const float wgt = (s_l[w] > 0.0f) ? ex2(s_m[w] - m_tot) : 0.0f;
-        l_tot += s_l[w] * wgt;
+        l_tot += s_l[w] * wgt;      // (SCORED: a mass that is NaN makes the sum NaN with any weight)
         const float4 a = *reinterpret_cast<const float4*>(&s_acc[w][8 * lane]), b = *reinterpret_cast<const float4*>(&s_acc[w][8 * lane + 4]);
         acc[0] += a.x * wgt; acc[1] += a.y * wgt; acc[2] += a.z * wgt; acc[3] += a.w * wgt;
         acc[4] += b.x * wgt; acc[5] += b.y * wgt; acc[6] += b.z * wgt; acc[7] += b.w * wgt;
@@ -1540,6 +1561,15 @@ __global__ void __launch_bounds__(MW * 32) tq4_attention_merge_kernel(const Stre
     if (!p.natural) {
         butterfly8<5>(acc, lane);
         sign8(acc, lane);
+    }
+    if (SCORED) {
+        bool fine = is_finite(l_tot);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) fine = fine && is_finite(acc[j]);
+        if (!__all_sync(0xffffffffu, fine)) {
+            const ScoredRow row = {&p.layout, &p.batch, &p.sc, p.q_in, p.io_bf16, p.num_q_heads, p.gqa};
+            scored_row_whole(row, r, tok - p.batch.query_start_loc[r], q_head, acc);
+        }
     }
     uint32_t gate[4];
     load_gate8(p.og, out_base, lane, gate);
@@ -1868,11 +1898,11 @@ static warp34_attention_batch batch_part(const warp34_attention_batch* batch, in
 
 // The merge behind a streaming kernel.  Few rows with hundreds of partials each (one long sequence): 32 warps per row
 // instead of 4.
-template <bool PARTIAL_OUT>
+template <bool PARTIAL_OUT, bool SCORED = false>
 static int launch_merge(const StreamParams& p, long long rows, cudaStream_t st) {
     const bool wide = rows * 4 < (long long)p.num_warps / 8;
-    return wide ? launch_behind(tq4_attention_merge_kernel<PARTIAL_OUT, 32>, (unsigned)rows, 1024, 0, st, p)
-                : launch_behind(tq4_attention_merge_kernel<PARTIAL_OUT, 4>, (unsigned)rows, 128, 0, st, p);
+    return wide ? launch_behind(tq4_attention_merge_kernel<PARTIAL_OUT, 32, SCORED>, (unsigned)rows, 1024, 0, st, p)
+                : launch_behind(tq4_attention_merge_kernel<PARTIAL_OUT, 4, SCORED>, (unsigned)rows, 128, 0, st, p);
 }
 
 }  // namespace w34
@@ -2043,10 +2073,12 @@ static bool takes_kv8_chunk_path(uint64_t flags, const warp34_kv_layer_layout* l
 // force: -1 = dispatch by batch geometry and flags; otherwise the kernel family the reference's
 // test selector names: 0 = the row-group kernels (8 query rows per item), 1 = the CTA-pair
 // prefill kernel, 2 = the tcgen05 prefill kernel.
+// sc != nullptr: scored attention, on the SCORED builds of the eight-row stream kernels and of the CTA-pair kernel (no gate, no triples, no
+// fast flag), and on scored_rows_kernel where those do not serve a call.
 static int launch_attention(const warp34_exec* ex, const warp34_kv_layer_layout* layout,
                             const warp34_attention_batch* batch, const void* q_in, void* attn_out,
                             float* triple_out, int num_q_heads, int io_bf16 = 0, int force = -1,
-                            const OutputGate* gate = nullptr) {
+                            const OutputGate* gate = nullptr, const ScoreChange* sc = nullptr) {
     OutputGate og;
     og.gate = gate != nullptr ? gate->gate : nullptr;
     og.mode = gate != nullptr ? gate->mode : 0;
@@ -2065,15 +2097,29 @@ static int launch_attention(const warp34_exec* ex, const warp34_kv_layer_layout*
             const Kv8Route route = kv8_chunk_route(ex, layout, batch, q_in, num_q_heads, io_bf16, dev->sm_count);
             if (route != kKv8Stream) {
                 const int skip_rows = route == kKv8Both ? kKv8ShortRows : 0;
+                if (sc != nullptr) {
+                    rc = layout->k_format == WARP34_KV_FORMAT_FP8_E4M3
+                             ? launch_prefill_pair<WARP34_KV_FORMAT_FP8_E4M3, true>(ex, layout, batch, q_in, attn_out, num_q_heads, io_bf16, og, dev->sm_count, skip_rows, *sc)
+                             : launch_prefill_pair<WARP34_KV_FORMAT_Q8_0, true>(ex, layout, batch, q_in, attn_out, num_q_heads, io_bf16, og, dev->sm_count, skip_rows, *sc);
+                } else {
                 rc = layout->k_format == WARP34_KV_FORMAT_FP8_E4M3
                          ? launch_prefill_pair<WARP34_KV_FORMAT_FP8_E4M3>(ex, layout, batch, q_in, attn_out, num_q_heads, io_bf16, og, dev->sm_count, skip_rows)
                          : launch_prefill_pair<WARP34_KV_FORMAT_Q8_0>(ex, layout, batch, q_in, attn_out, num_q_heads, io_bf16, og, dev->sm_count, skip_rows);
+                }
                 if (rc != 0 || route == kKv8Pair) return rc;
                 const warp34_attention_batch rest = kv8_short_part(batch, num_q_heads / layout->local_kv_heads);
                 bool taken = false;
-                rc = launch_kv8_stream(ex, layout, &rest, q_in, attn_out, num_q_heads, io_bf16, &taken, &og);
+                rc = launch_kv8_stream(ex, layout, &rest, q_in, attn_out, num_q_heads, io_bf16, &taken, &og, sc);
                 return rc != 0 || taken ? rc : (int)cudaErrorInvalidValue;      // (kv8_chunk_route has seen that it is taken)
             }
+        }
+        if (sc != nullptr) {
+            bool taken = false;
+            if ((ex->flags & WARP34_B200_EXEC_FLAG_PRECISE_ATTENTION) == 0 && kv8_stream_ok(ex, layout, batch, q_in, io_bf16)) {
+                const int rc = launch_kv8_stream(ex, layout, batch, q_in, attn_out, num_q_heads, io_bf16, &taken, nullptr, sc);
+                if (rc != 0 || taken) return rc;
+            }
+            return launch_scored_rows(ex, layout, batch, *sc, q_in, attn_out, num_q_heads, io_bf16);
         }
         const int rc8 = launch_kv8_attention(ex, layout, batch, q_in, attn_out, num_q_heads, io_bf16,
                                              (ex->flags & WARP34_B200_EXEC_FLAG_PRECISE_ATTENTION) == 0 && force <= 0);
@@ -2095,8 +2141,11 @@ static int launch_attention(const warp34_exec* ex, const warp34_kv_layer_layout*
     const bool chunk_geometry_ok = stream_layout_ok(layout) && batch->max_blocks_per_req > 0 && gqa <= kPpCtaRows;
     if (force >= 1 && (!chunk_geometry_ok || triple_out != nullptr)) return (int)cudaErrorNotSupported;
     if (force >= 1 || (force < 0 && triple_out == nullptr && takes_prefill_path(ex->flags, layout, batch, gqa))) {
-        const bool tc = force == 2 || (force < 0 && (ex->flags & (WARP34_B200_EXEC_FLAG_FAST_ATTENTION |
-                                                                  WARP34_B200_EXEC_FLAG_TCGEN05_VERIFY)) != 0);
+        const bool tc = sc == nullptr && (force == 2 || (force < 0 && (ex->flags & (WARP34_B200_EXEC_FLAG_FAST_ATTENTION |
+                                                                  WARP34_B200_EXEC_FLAG_TCGEN05_VERIFY)) != 0));
+        if (sc != nullptr) {
+            return launch_prefill_pair<WARP34_KV_FORMAT_TQ4, true>(ex, layout, batch, q_in, attn_out, num_q_heads, io_bf16, og, dev->sm_count, 0, *sc);
+        }
         if (tc) {
             if (layout->local_kv_heads > 65535) return (int)cudaErrorInvalidValue;
             if ((size_t)dev->smem_optin < kTcSmemBytes) return (int)cudaErrorNotSupported;
@@ -2129,7 +2178,7 @@ static int launch_attention(const warp34_exec* ex, const warp34_kv_layer_layout*
 
     // Streaming path: canonical layout, scratch that holds the plan plus at least one partial
     // per item and per worker, unit count within int32.
-    const bool fast = (ex->flags & WARP34_B200_EXEC_FLAG_FAST_ATTENTION) != 0;
+    const bool fast = sc == nullptr && (ex->flags & WARP34_B200_EXEC_FLAG_FAST_ATTENTION) != 0;
     const int workers_per_cta = fast ? kFastWarps : kExactWarps;
     const size_t slot_bytes = (size_t)kPartialFloats * sizeof(float);
     const long long full_workers = (long long)dev->sm_count * workers_per_cta;
@@ -2139,7 +2188,7 @@ static int launch_attention(const warp34_exec* ex, const warp34_kv_layer_layout*
     if (qfrag_items(layout, batch, gqa) > 0x3fffffffll) return (int)cudaErrorInvalidValue;
 
     const int tile_rows = xt_rows(batch, gqa);
-    if (stream_ok && force < 0 && takes_tiles(ex, layout, batch, num_q_heads, tile_rows, dev->sm_count)) {
+    if (stream_ok && force < 0 && sc == nullptr && takes_tiles(ex, layout, batch, num_q_heads, tile_rows, dev->sm_count)) {
         cudaStream_t st = (cudaStream_t)ex->stream;
         const long long items = items_bound(layout, batch, num_q_heads, tile_rows);
         const long long q_items = (long long)batch->num_reqs * layout->local_kv_heads;
@@ -2196,6 +2245,7 @@ static int launch_attention(const warp34_exec* ex, const warp34_kv_layer_layout*
     }
     if (!stream_ok || workers < workers_per_cta) {
         if (triple_out != nullptr) return (int)cudaErrorNotSupported;
+        if (sc != nullptr) return launch_scored_rows(ex, layout, batch, *sc, q_in, attn_out, num_q_heads, io_bf16);
         return launch_scalar(ex, layout, batch, q_in, attn_out, num_q_heads, io_bf16, &og);
     }
 
@@ -2238,14 +2288,16 @@ static int launch_attention(const warp34_exec* ex, const warp34_kv_layer_layout*
         p.qfrag = reinterpret_cast<uint32_t*>(p.scratch + plan + (size_t)p.max_slots * slot_bytes);
         p.smem_bytes = (uint32_t)smem;
         p.q_groups_max = (int)(q_items / ((long long)reqs * layout->local_kv_heads));
+        if (sc != nullptr) p.sc = *sc;
         rc = launch_behind(tq4_attention_plan_kernel, 1 + (unsigned)q_items, q_items > 0 ? kPlanThreads : 32, 0, st, p);
         if (rc != 0) return rc;
-        if (fast) tq4_attention_stream_kernel<kFastStages, kFastWarps><<<grid, kFastWarps * 32, smem, st>>>(p);
+        if (sc != nullptr) rc = launch_behind(four_rows ? tq4_attention_stream_exact_kernel<false, kRowsByPlan, true> : tq4_attention_stream_exact_kernel<false, kEightRows, true>, (unsigned)grid, kXThreads, smem, st, p);
+        else if (fast) tq4_attention_stream_kernel<kFastStages, kFastWarps><<<grid, kFastWarps * 32, smem, st>>>(p);
         else rc = launch_behind(four_rows ? tq4_attention_stream_exact_kernel<false, kRowsByPlan> : tq4_attention_stream_exact_kernel<false, kEightRows>, (unsigned)grid, kXThreads, smem, st, p);
         // rows of the merge: every token of the batch, or (a part) as many as the part can hold, counted
         // from its first token
         const long long rows = (long long)p.batch.total_tokens * num_q_heads;
-        if (rc == 0) rc = triple_out != nullptr ? launch_merge<true>(p, rows, st) : launch_merge<false>(p, rows, st);
+        if (rc == 0) rc = sc != nullptr ? launch_merge<false, true>(p, rows, st) : triple_out != nullptr ? launch_merge<true>(p, rows, st) : launch_merge<false>(p, rows, st);
         if (rc != 0) return rc;
         rc = (int)cudaGetLastError();
         if (rc != 0) return rc;

@@ -135,7 +135,7 @@ __device__ __forceinline__ void x_stage_output(const XWarp& x, float* stage_o, f
 
 // Streams units [pg0, pg0 + n_here) of one work item.  `load_query(qb, ql)` runs once, after the first copies are on their way.
 // Leaves the accumulators, running maxima and row masses of this lane's rows (2 tig, 2 tig + 1); x.failed when a wait gave up.
-template <bool SPARSE, bool FOUR, class LoadQuery>
+template <bool SPARSE, bool FOUR, bool SCORED, class LoadQuery>
 __device__ __forceinline__ void x_stream(const StreamParams& p, XWarp& x, int r, const ReqGeom& g, int kv_head, int group, int pg0,
                                          int n_here, LoadQuery load_query, float (&o)[16][4], float (&m_run)[2], float (&l_row)[2]) {
     const int lane = x.lane, gid = x.gid, tig = x.tig, key_a = x.key_a, kv0 = x.kv0;
@@ -210,14 +210,20 @@ __device__ __forceinline__ void x_stream(const StreamParams& p, XWarp& x, int r,
     // limits of this lane's two query rows (2 tig, 2 tig + 1)
     int rmax[2], rmin[2];
     bool rvalid[2];
+    float slope[2] = {0.0f, 0.0f};      // SCORED: of the lane's two rows
+    int q_pos[2] = {0, 0};
 #pragma unroll
     for (int y = 0; y < 2; ++y) {
         const int row = group * kRowsPerGroup + 2 * (FOUR ? tig & 1 : tig) + y;
         const int q_off = row / p.gqa;
         rvalid[y] = row < rows_in_req &&
                     (p.batch.valid_token_mask == nullptr || p.batch.valid_token_mask[g.q_start + q_off] != 0);
-        rmax[y] = rvalid[y] ? row_max_kv(p.batch, g, q_off) : -1;
-        rmin[y] = rvalid[y] ? row_min_kv(p.batch, g, q_off) : 0x7fffffff;
+        rmax[y] = rvalid[y] ? row_last_key<SCORED>(p.batch, p.sc, g, q_off) : -1;
+        rmin[y] = rvalid[y] ? row_first_key<SCORED>(p.batch, p.sc, g, q_off) : 0x7fffffff;
+        if (SCORED) {
+            slope[y] = rvalid[y] ? row_slope(p.sc, kv_head * p.gqa + row - q_off * p.gqa) : 0.0f;
+            q_pos[y] = g.ctx_before + q_off;
+        }
     }
     // keys in [safe_lo, safe_hi] are visible to every valid row of the group
     int safe_hi = min(rvalid[0] ? rmax[0] : 0x7fffffff, rvalid[1] ? rmax[1] : 0x7fffffff);
@@ -307,6 +313,14 @@ __device__ __forceinline__ void x_stream(const StreamParams& p, XWarp& x, int r,
                 for (int c = 0; c < 4; ++c) pr[y][c] += __shfl_xor_sync(0xffffffffu, pr[y][c], 2);
             }
             const int kv_base = (pg0 + 2 * st + y) << 4;
+            if (SCORED) {
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    const float away = (float)(q_pos[c] - (kv_base + key_a));
+                    pr[y][c] = changed_score(p.sc, pr[y][c], slope[c], away);
+                    pr[y][2 + c] = changed_score(p.sc, pr[y][2 + c], slope[c], away - 4.0f);
+                }
+            }
             int pos_a = kv_base + key_a, pos_b = pos_a + 4;
             if (SPARSE) {     // position of the first row of the two groups this lane's keys sit in
                 const uint32_t pw = kst + kHalfBytes;
@@ -391,6 +405,10 @@ __device__ __forceinline__ void x_stream(const StreamParams& p, XWarp& x, int r,
             const float db1 = zb ? 0.0f : __half2float(__ushort_as_half((unsigned short)(vb16 >> 16)));
             pd[0][0] = pr[y][0] * da0; pd[0][1] = pr[y][1] * da0; pd[0][2] = pr[y][2] * db0; pd[0][3] = pr[y][3] * db0;
             pd[1][0] = pr[y][0] * da1; pd[1][1] = pr[y][1] * da1; pd[1][2] = pr[y][2] * db1; pd[1][3] = pr[y][3] * db1;
+            if (SCORED && !full[y]) {      // a key that only one of the rows sees: its scales may be NaN to the other
+#pragma unroll
+                for (int c = 0; c < 4; ++c) if (pr[y][c] == 0.0f) pd[0][c] = pd[1][c] = 0.0f;
+            }
         };
         // code bytes of step i4: byte t of ab[0] -> (V[ka][e = 2 t], V[kb][e = 2 t]), of ab[1] -> e = 2 t + 1
         auto code_pairs = [&](uint32_t vr, int i4, uint32_t (&ab)[2], uint32_t (&cd)[2]) {
@@ -503,7 +521,7 @@ struct XHeld {
 // FOUR: items of at most four query rows.  The N = 8 columns of an MMA hold their values and, beside them, their rounding residuals (of the
 // query for the scores, of the weights for the output), so that one MMA does what takes two with eight rows: 48 a page instead of 80,
 // with the tensor pipe at 45 % and its issue among the stalls.
-template <bool SPARSE, bool FOUR>
+template <bool SPARSE, bool FOUR, bool SCORED>
 __device__ __forceinline__ int x_share(const StreamParams& p, XWarp& x, PlanHeader* hdr, int u, int u_end, int w_global, bool neighbours,
                                        float* ring_gen, XHeld& held_by) {
     const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
@@ -533,7 +551,7 @@ __device__ __forceinline__ int x_share(const StreamParams& p, XWarp& x, PlanHead
         const ReqGeom g = stream_req(p, r);
         float o[16][4], m_run[2], l_row[2];
         const uint32_t* qf = p.qfrag + ((size_t)(r * p.layout.local_kv_heads + kv_head) * p.q_groups_max + group) * (kQFragWords * 32) + (FOUR ? lane & 15 : lane);
-        x_stream<SPARSE, FOUR>(p, x, r, g, kv_head, group, pg0, n_here,
+        x_stream<SPARSE, FOUR, SCORED>(p, x, r, g, kv_head, group, pg0, n_here,
                          // (not __ldg: the plan kernel was still writing these words when this one started)
                          [&](uint32_t (&qb)[16][2], uint32_t (&ql)[FOUR ? 1 : 16][2]) { x_load_query<FOUR>([&](int i) { return qf[i * 32]; }, qb, ql); },
                          o, m_run, l_row);
@@ -581,7 +599,7 @@ __device__ __forceinline__ int x_share(const StreamParams& p, XWarp& x, PlanHead
 // Rows per item: eight, four, or four where the plan found that no request has more (kRowsByPlan: a batch that declares up to four, but a
 // request may hold more than its batch declares, and an item of eight still takes all of its rows then).
 enum ItemRows { kEightRows, kFourRows, kRowsByPlan };
-template <bool SPARSE, ItemRows ROWS>
+template <bool SPARSE, ItemRows ROWS, bool SCORED = false>
 __global__ void __launch_bounds__(kXThreads, 1) tq4_attention_stream_exact_kernel(const StreamParams p) {
     extern __shared__ __align__(1024) uint8_t smem[];
     const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
@@ -626,10 +644,10 @@ __global__ void __launch_bounds__(kXThreads, 1) tq4_attention_stream_exact_kerne
     const int u_end = min(u + per, total_units);
     int held;
     if constexpr (ROWS == kRowsByPlan) {
-        held = plan_array(p.scratch, 2, R)[R] == 0 ? x_share<SPARSE, true>(p, x, hdr, u, u_end, w_global, neighbours, ring_gen, held_by)
-                                                   : x_share<SPARSE, false>(p, x, hdr, u, u_end, w_global, neighbours, ring_gen, held_by);
+        held = plan_array(p.scratch, 2, R)[R] == 0 ? x_share<SPARSE, true, SCORED>(p, x, hdr, u, u_end, w_global, neighbours, ring_gen, held_by)
+                                                   : x_share<SPARSE, false, SCORED>(p, x, hdr, u, u_end, w_global, neighbours, ring_gen, held_by);
     } else {
-        held = x_share<SPARSE, ROWS == kFourRows>(p, x, hdr, u, u_end, w_global, neighbours, ring_gen, held_by);
+        held = x_share<SPARSE, ROWS == kFourRows, SCORED>(p, x, hdr, u, u_end, w_global, neighbours, ring_gen, held_by);
     }
     if (!neighbours) return;
     float* partials = reinterpret_cast<float*>(p.scratch + plan_bytes(R));
@@ -648,9 +666,9 @@ __global__ void __launch_bounds__(kXThreads, 1) tq4_attention_stream_exact_kerne
         const int slot = (int)blockIdx.x * kExactWarps + first + item;
         if (item >= 0 && slot + (end - first) <= p.max_slots) {
             float m_tot = -1e30f, l_tot = 0.0f, v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-            for (int w = first; w < end; ++w) if (held_by.l[w][wid] > 0.0f) m_tot = fmaxf(m_tot, held_by.m[w][wid]);
+            for (int w = first; w < end; ++w) if (SCORED ? held_by.l[w][wid] != 0.0f : held_by.l[w][wid] > 0.0f) m_tot = fmaxf(m_tot, held_by.m[w][wid]);
             for (int w = first; w < end; ++w) {
-                const float l = held_by.l[w][wid], wgt = l > 0.0f ? ex2(held_by.m[w][wid] - m_tot) : 0.0f;
+                const float l = held_by.l[w][wid], wgt = (SCORED ? l != 0.0f : l > 0.0f) ? ex2(held_by.m[w][wid] - m_tot) : 0.0f;
                 l_tot += l * wgt;
                 const float4* src = reinterpret_cast<const float4*>(smem + held_by.ring[w] + (wid * kHeadDim + 8 * lane) * 4);
                 const float4 a = src[0], b = src[1];

@@ -69,6 +69,11 @@ class PeerMailboxes(C.Structure):
                 ("wait_limit", C.c_uint32), ("reserved", C.c_uint32)]
 
 
+class ScoreChange(C.Structure):
+    _fields_ = [("distance_slopes", C.c_void_p), ("key_begin", C.c_void_p), ("key_end", C.c_void_p), ("softcap", C.c_float),
+                ("reserved", C.c_int32)]
+
+
 class QkNormRopeArgs(C.Structure):
     _fields_ = [(n, C.c_void_p) for n in ("q_in", "k_in", "q_out", "k_out", "gate_out", "q_norm_w", "k_norm_w", "positions", "inv_freq",
                                           "valid_token_mask")] + \
@@ -79,7 +84,7 @@ class QkNormRopeArgs(C.Structure):
                [("rms_eps", C.c_float), ("weight_offset", C.c_float)]
 
 
-assert C.sizeof(PeerMailboxes) == 168 and C.sizeof(QkNormRopeArgs) == 168
+assert C.sizeof(PeerMailboxes) == 168 and C.sizeof(QkNormRopeArgs) == 168 and C.sizeof(ScoreChange) == 32
 assert C.sizeof(Exec) == 32 and C.sizeof(KvLayerLayout) == 104 and C.sizeof(AttentionBatch) == 96
 
 _P = C.POINTER
@@ -128,6 +133,9 @@ _KERNEL_SIGS = {
     "warp34_paged_attention_bf16": (C.c_int, [_P(Exec), _P(KvLayerLayout), _P(AttentionBatch),
                                               C.c_void_p, C.c_void_p, C.c_int]),
     "warp34_paged_attention_bf16_scratch_bytes": (C.c_size_t, [_P(KvLayerLayout), _P(AttentionBatch), C.c_int]),
+    "warp34_paged_attention_scored_f16": (C.c_int, [_P(Exec), _P(KvLayerLayout), _P(AttentionBatch), _P(ScoreChange), C.c_void_p, C.c_void_p, C.c_int]),
+    "warp34_paged_attention_scored_bf16": (C.c_int, [_P(Exec), _P(KvLayerLayout), _P(AttentionBatch), _P(ScoreChange), C.c_void_p, C.c_void_p, C.c_int]),
+    "warp34_paged_attention_scored_scratch_bytes": (C.c_size_t, [_P(KvLayerLayout), _P(AttentionBatch), C.c_int]),
     "warp34_qk_norm_rope_f16": (C.c_int, [_P(Exec), _P(QkNormRopeArgs)]),
     "warp34_qk_norm_rope_bf16": (C.c_int, [_P(Exec), _P(QkNormRopeArgs)]),
     "warp34_kv_cache_read_f16": (C.c_int, [_P(Exec), _P(KvLayerLayout), _P(AttentionBatch), C.c_void_p, C.c_void_p, C.c_int, C.c_int]),

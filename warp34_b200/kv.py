@@ -477,6 +477,29 @@ def _require(ok, what):
         raise ValueError(what)
 
 
+def paged_attention_scored(ex, layer, batch, q, out, num_q_heads, softcap=0.0, slopes=None, key_begin=None, key_end=None, lib=None):
+    """warp34_paged_attention_scored_f16 / _bf16 (by q's type): attention with capped scores (softcap), a penalty of slopes[head] per key of
+    distance, and a range of keys [key_begin, key_end) per token (int32 [tokens]; key_end in place of causality)."""
+    lib = lib or ffi.kernels()
+    dtype, n = q.dtype, batch.desc.total_tokens
+    _require(dtype in (torch.float16, torch.bfloat16) and out.dtype == dtype and q.is_contiguous() and out.is_contiguous() and
+             q.numel() >= n * num_q_heads * 256 and out.numel() >= n * num_q_heads * 256,
+             f"paged_attention_scored: contiguous fp16 or bf16 q and out of [{n}, {num_q_heads}, 256]")
+    c = ffi.ScoreChange(None, None, None, softcap, 0)
+    if slopes is not None:
+        _require(slopes.dtype == torch.float32 and slopes.numel() == num_q_heads and slopes.is_contiguous(), f"slopes: fp32 [{num_q_heads}]")
+        c.distance_slopes = slopes.data_ptr()
+    if key_begin is not None:
+        _require(key_begin.dtype == torch.int32 and key_begin.numel() >= n and key_begin.is_contiguous(), f"key_begin: int32 [{n}]")
+        c.key_begin = key_begin.data_ptr()
+    if key_end is not None:
+        _require(key_end.dtype == torch.int32 and key_end.numel() >= n and key_end.is_contiguous(), f"key_end: int32 [{n}]")
+        c.key_end = key_end.data_ptr()
+    fn = lib.warp34_paged_attention_scored_f16 if dtype == torch.float16 else lib.warp34_paged_attention_scored_bf16
+    _check(fn(C.byref(ex.ex), C.byref(layer.layout), C.byref(batch.desc), C.byref(c), q.data_ptr(), out.data_ptr(), num_q_heads),
+           "warp34_paged_attention_scored")
+
+
 def _head_rows(t, dtype, heads, width, what):
     """Checks that t is [tokens, heads, width] with heads next to each other; returns its token stride."""
     _require(t.dtype == dtype and t.dim() == 3 and t.shape[2] == width and (heads is None or t.shape[1] == heads),
