@@ -5,12 +5,18 @@
 //
 // in fp32, rounded once to the output type.
 //
-// Eight lanes hold a row, a warp four rows of neighbouring tokens.  The output is three quarters of the bytes, so it decides the
-// layout: a lane ends with 16-byte chunks j + 8 i of its row, eight lanes write whole 128-byte lines.  TQ4 rows start in the other
-// layout, quads (4 columns, 2 bytes of codes): there five levels of the transform are register arithmetic, the columns then
-// change lanes through shared memory once, and the other three are register arithmetic again.  Both scales of a row meet in
-// the last level, whose butterfly is d0 a +- d1 b.  Codes go through a table of value pairs by byte, 16 copies of 8 bytes.
-// Bound by HBM and, on TQ4 rows, close to it by the shared-memory pipe (24 wavefronts a row).
+// A warp holds a row (and, where there are tokens enough, four rows of neighbouring heads on their way at once).  TQ4: column 16 a + b of
+// the row is element (b, a) of a 16 x 16 matrix, and the transform a product from either side, both on the tensor cores
+// (mma.sync m16n8k16, fp32 accumulators) with a matrix of +-1:
+//     Z = (H / 256) (16 X),  U = Z (1 x H8),  Y = d0 U0 +- d1 U1
+// with U0, U1 the 8-point transforms of the two halves of Z's columns, which have a scale each, and the last level, where they meet, in fp32.
+// X comes as fp16 value and residual from a table by code byte (22 bits of a centroid), Z is split the same way: eight products a row.
+// The accumulators of the first are the A fragments of the second as they lie in the lanes; columns of the first +-1 matrix are ordered so
+// that a lane's elements are four neighbouring columns (two code bytes).  The rounded row passes through shared memory (stmatrix,
+// transposed), so that a lane stores 16 bytes.  (With movmatrix instead of that, 8 bytes a lane: 55 us.)
+// (Eight lanes to a row, the transform in packed fp32 arithmetic and its columns changing lanes through shared memory: 67 us instead of
+// 55 for 35065 tokens of 4 heads, at 40 shared-memory wavefronts and 168 instructions a row.)
+// Bound by instruction issue (118 a row, 60 % of the slots) and by the latency of the rows' loads (a third of the stalls); HBM is at 26 %.
 #include "tq4_common.cuh"
 
 #include <cuda_bf16.h>
@@ -19,8 +25,9 @@
 namespace w34 {
 
 constexpr int kReadWarps = 8;
-constexpr int kReadTableBytes = 256 * 128;
-constexpr int kReadTurnBytes = kReadWarps * 4 * 1024;      // four rows a warp change lanes at once
+constexpr int kReadTq4Blocks = 4;              // resident blocks an SM that a grid is sized for
+constexpr int kReadRows = 4;                   // rows of a warp on their way at once: heads of one token
+constexpr int kReadTableBytes = 256 * 128;     // byte -> (value pair, residual pair), 16 copies
 
 struct ReadParams {
     warp34_kv_layer_layout layout;
@@ -30,7 +37,7 @@ struct ReadParams {
     int first, sides;           // 0: K first; how many of the two are read
     int aligned;                // output rows start on 16-byte boundaries
     int rows_aligned;           // BF16 rows do
-    long long units;            // sides x kv heads x groups of four tokens
+    int tokens_per_warp;
 };
 
 template <bool BF16>
@@ -42,209 +49,227 @@ __device__ __forceinline__ uint32_t read_narrow(float a, float b) {
     const __half2 v = __floats2half2_rn(a, b);
     return *reinterpret_cast<const uint32_t*>(&v);
 }
-__device__ __forceinline__ void read_store8(uint16_t* dst, int aligned, const uint32_t (&w)[4]) {
-    if (aligned) {
-        *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
-    } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) { dst[2 * i] = (uint16_t)w[i]; dst[2 * i + 1] = (uint16_t)(w[i] >> 16); }
-    }
+__device__ __forceinline__ void read_mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-
-// Place of a 16-byte quad of a row while the columns change lanes: conflict-free for quads stored at 2 (j + 8 (l / 2)) + l % 2 by lane l
-// and for the pairs 2 c, 2 c + 1 of chunk c = j + 8 i read by lane j.
-__device__ __forceinline__ uint32_t read_quad_place(uint32_t u) { return u ^ ((u >> 3) & 1u) ^ (((u >> 4) & 3u) << 1); }
-
-typedef unsigned long long F2;
-__device__ __forceinline__ F2 f2(float a, float b) { return (F2)__float_as_uint(a) | ((F2)__float_as_uint(b) << 32); }
-__device__ __forceinline__ float f2x(F2 p) { return __uint_as_float((uint32_t)p); }
-__device__ __forceinline__ float f2y(F2 p) { return __uint_as_float((uint32_t)(p >> 32)); }
-__device__ __forceinline__ F2 f2add(F2 a, F2 b) {
-    F2 r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
+__device__ __forceinline__ void read_mma_zero(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
 }
-__device__ __forceinline__ F2 f2mul(F2 a, F2 b) {
-    F2 r;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
+__device__ __forceinline__ void read_mma8(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t b0) {
+    asm("mma.sync.aligned.m16n8k8.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5}, {%6}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(b0));
 }
-__device__ __forceinline__ F2 f2fma(F2 a, F2 b, F2 c) {
-    F2 r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-    return r;
+__device__ __forceinline__ void read_mma8_zero(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t b0) {
+    asm("mma.sync.aligned.m16n8k8.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5}, {%6}, {%7,%7,%7,%7};"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3]) : "r"(a0), "r"(a1), "r"(b0), "f"(0.0f));
 }
-// Butterflies over pair-index bit d of 16 packed pairs.
-__device__ __forceinline__ void read_level(F2 (&x)[16], int d, F2 minus_one) {
-#pragma unroll
-    for (int k = 0; k < 16; ++k) {
-        if (k & d) continue;
-        const F2 a = x[k], b = x[k | d];
-        x[k] = f2add(a, b);
-        x[k | d] = f2fma(b, minus_one, a);
-    }
+__device__ __forceinline__ uint32_t read_half2(float a, float b) {
+    const __half2 v = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&v);
 }
-
-// Address of the row of token `tok` (K or V), or 0: the row takes no part.
-__device__ __forceinline__ uint64_t read_row_address(const ReadParams& p, int tok, int head, int side) {
+// a and b as fp16 pairs of values and of residuals.  The value is cut off, not rounded (one instruction, and exactly what the pair then holds):
+// the residual is below 2^-10 of it and keeps 11 bits of its own.
+__device__ __forceinline__ void read_split(float a, float b, uint32_t& value, uint32_t& residual) {
+    const float va = __uint_as_float(__float_as_uint(a) & 0xffffe000u), vb = __uint_as_float(__float_as_uint(b) & 0xffffe000u);
+    value = read_half2(va, vb);
+    residual = read_half2(a - va, b - vb);
+}
+// Entries (i, j0), (i, j1) of the 16-point Walsh-Hadamard matrix times `scale`, as an fp16 pair.
+__device__ __forceinline__ uint32_t read_hadamard(int i, int j0, int j1, float scale) {
+    return read_half2((__popc(i & j0) & 1) ? -scale : scale, (__popc(i & j1) & 1) ? -scale : scale);
+}
+// Page and offset of token `tok`, or a negative page: the token takes no part.
+__device__ __forceinline__ int read_place(const ReadParams& p, int tok, int& off) {
     const warp34_attention_batch& b = p.batch;
-    if (tok >= b.total_tokens || (b.valid_token_mask != nullptr && b.valid_token_mask[tok] == 0)) return 0;
-    const int r = find_request(b.query_start_loc, b.num_reqs, tok);
-    if (r < 0 || (b.valid_req_mask != nullptr && b.valid_req_mask[r] == 0)) return 0;
-    int page, off;
-    if (b.write_slot_mapping != nullptr) {
+    if (b.valid_token_mask != nullptr && b.valid_token_mask[tok] == 0) return -1;
+    if (b.write_slot_mapping != nullptr && b.valid_req_mask == nullptr) {
+        if (tok < b.query_start_loc[0] || tok >= b.query_start_loc[b.num_reqs]) return -1;
+    }
+    const bool by_slot = b.write_slot_mapping != nullptr;
+    int r = 0;
+    if (!by_slot || b.valid_req_mask != nullptr) {
+        r = find_request(b.query_start_loc, b.num_reqs, tok);
+        if (r < 0 || (b.valid_req_mask != nullptr && b.valid_req_mask[r] == 0)) return -1;
+    }
+    int page;
+    if (by_slot) {
         const int slot = b.write_slot_mapping[tok];
-        if (slot < 0) return 0;
+        if (slot < 0) return -1;
         page = slot >> 4;
         off = slot & 15;
     } else {
         const int q_len = b.query_start_loc[r + 1] - b.query_start_loc[r];
         const int pos = (b.context_lens_before != nullptr ? b.context_lens_before[r] : b.seq_lens_after[r] - q_len) + (tok - b.query_start_loc[r]);
-        if (pos < 0 || (pos >> 4) >= b.max_blocks_per_req) return 0;
+        if (pos < 0 || (pos >> 4) >= b.max_blocks_per_req) return -1;
         page = block_table_page(b.block_tables + (size_t)r * b.max_blocks_per_req, pos >> 4, b.max_blocks_per_req, kInRead);
         off = pos & 15;
     }
-    page = pool_page(page, kInRead);
+    return pool_page(page, kInRead);
+}
+__device__ __forceinline__ const uint8_t* read_row(const ReadParams& p, int page, int off, int head, int side) {
     const warp34_kv_layer_layout& l = p.layout;
-    return side == 0 ? l.k_base + (uint64_t)page * l.k_page_stride_bytes + (uint64_t)head * l.k_head_stride_bytes + (uint64_t)off * l.k_token_stride_bytes
-                     : l.v_base + (uint64_t)page * l.v_page_stride_bytes + (uint64_t)head * l.v_head_stride_bytes + (uint64_t)off * l.v_token_stride_bytes;
+    const uint64_t at = side == 0 ? l.k_base + (uint64_t)page * l.k_page_stride_bytes + (uint64_t)head * l.k_head_stride_bytes + (uint64_t)off * l.k_token_stride_bytes
+                                  : l.v_base + (uint64_t)page * l.v_page_stride_bytes + (uint64_t)head * l.v_head_stride_bytes + (uint64_t)off * l.v_token_stride_bytes;
+    return reinterpret_cast<const uint8_t*>((uintptr_t)at);
 }
 
-// Unit: four tokens of one head, K or V.  Units of a side follow each other by token group, then head.
-struct ReadUnit { int tok, head, side; uint64_t row; };
-__device__ __forceinline__ ReadUnit read_unit(const ReadParams& p, long long u) {
-    ReadUnit x;
-    const int heads = p.layout.local_kv_heads;
-    const long long g = u / p.sides;
-    x.side = p.first + (int)(u - g * p.sides);
-    const long long group = g / heads;
-    x.head = (int)(g - group * heads);
-    x.tok = (int)(4 * group) + (int)((threadIdx.x & 31) >> 3);
-    x.row = read_row_address(p, x.tok, x.head, x.side);
-    return x;
-}
-
-template <bool BF16>
-__global__ void __launch_bounds__(kReadWarps * 32, 3) kv_read_tq4_kernel(const ReadParams p) {
-    extern __shared__ __align__(128) uint8_t smem[];
-    const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5, j = lane & 7, r4 = lane >> 3;
-    for (int i = threadIdx.x; i < 256 * 16; i += kReadWarps * 32) {
-        const int byte = i >> 4;
-        *reinterpret_cast<float2*>(smem + byte * 128 + (i & 15) * 8) = make_float2(tq4_centroid(byte & 15), tq4_centroid(byte >> 4));
+// The tokens of a warp are neighbours, an equal share for every warp of the grid.  Its lanes look up 32 of their rows at once: looked up
+// one by one, a token's place cost as much as one and a half of its rows.
+struct ReadShare {
+    int first, end;
+    __device__ __forceinline__ explicit ReadShare(const ReadParams& p) {
+        const long long w = (long long)blockIdx.x * kReadWarps + (threadIdx.x >> 5), per = p.tokens_per_warp;
+        first = (int)min(w * per, (long long)p.batch.total_tokens);
+        end = (int)min((w + 1) * per, (long long)p.batch.total_tokens);
     }
-    // signs of this lane's output columns 8 (j + 8 i) + e as sign bits of packed pairs
-    uint32_t sign[16];
+};
+// Address of the row of token first + lane, or 0.
+__device__ __forceinline__ uint64_t read_rows_of(const ReadParams& p, int first, int end, int head, int side) {
+    const int tok = first + (int)(threadIdx.x & 31);
+    int off = 0;
+    const int page = tok < end ? read_place(p, tok, off) : -1;
+    return page < 0 ? 0 : (uint64_t)(uintptr_t)read_row(p, page, off, head, side);
+}
+
+// blockIdx.y: side x group of ROWS heads.
+template <bool BF16, int ROWS>
+__global__ void __launch_bounds__(kReadWarps * 32, kReadTq4Blocks) kv_read_tq4_kernel(const __grid_constant__ ReadParams p) {
+    __shared__ __align__(128) uint8_t table[kReadTableBytes];
+    __shared__ __align__(128) uint8_t turns[512 * kReadWarps];
+    const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5, gid = lane >> 2, tig = lane & 3;
+    {      // entry `threadIdx.x`; centroids x 16, so that their residuals are normal numbers
+        const float c0 = 16.0f * tq4_centroid(threadIdx.x & 15), c1 = 16.0f * tq4_centroid(threadIdx.x >> 4);
+        const uint32_t hi = read_half2(c0, c1);
+        const float2 hf = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+        const uint2 e = make_uint2(hi, read_half2(c0 - hf.x, c1 - hf.y));
+        static_assert(kReadWarps * 32 == 256, "one entry per thread");
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int c = 8 * (j + 8 * i);
-        const uint32_t m = c_sign_mask[c >> 5] >> (c & 31);
+        for (int i = 0; i < 16; ++i) *reinterpret_cast<uint2*>(table + threadIdx.x * 128 + ((i + threadIdx.x) & 15) * 8) = e;
+    }
+    // k position 2 t, 2 t + 1, 2 t + 8, 2 t + 9 of a product <-> b = 4 t .. 4 t + 3
+    auto order = [](int m) { return 4 * ((m & 7) >> 1) + (m & 1) + 2 * (m >> 3); };
+    uint32_t ha[4];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) sign[4 * i + k] = (((m >> (2 * k)) & 1u) << 15) | (((m >> (2 * k + 1)) & 1u) << 31);
+    for (int i = 0; i < 4; ++i) {      // A fragment: rows gid, gid + 8, k 2 tig (+ 8)
+        const int m = gid + 8 * (i & 1), k = 2 * tig + 8 * (i >> 1);
+        ha[i] = read_hadamard(m, order(k), order(k + 1), 1.0f / 256.0f);
+    }
+    const uint32_t hb = read_hadamard(gid, 2 * tig, 2 * tig + 1, 1.0f);
+    uint32_t sign[4];      // of columns 8 lane .. + 7, as the sign bits of packed pairs
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const uint32_t m = c_sign_mask[lane >> 2] >> (8 * (lane & 3) + 2 * k);
+        sign[k] = ((m & 1u) << 15) | ((m & 2u) << 30);
     }
     grid_dependency_wait();      // nothing above touches global memory
     grid_launch_dependents();
     __syncthreads();
-    const uint8_t* table = smem + 8 * (lane & 15);
-    uint8_t* turn = smem + kReadTableBytes + (wid * 4 + r4) * 1024;
-    const F2 minus_one = f2(-1.0f, -1.0f);
+    const uint32_t copy = 8u * (uint32_t)(lane & 15);
+    const int heads = p.layout.local_kv_heads, groups = (heads + ROWS - 1) / ROWS;
+    const int side = p.first + (int)blockIdx.y / groups, head0 = (int)blockIdx.y % groups * ROWS;
+    const uint64_t head_stride = side == 0 ? p.layout.k_head_stride_bytes : p.layout.v_head_stride_bytes;
+    const int n_rows = min(ROWS, heads - head0);
+    // The finished row passes through 512 bytes of this warp's: 16-byte chunk c (columns 8 c .. + 7) at place c ^ (c >> 3 & 1), free of bank
+    // conflicts for the matrices' rows (every other chunk) and for the lanes' chunks.
+    const uint32_t turn = (uint32_t)__cvta_generic_to_shared(turns) + 512u * (uint32_t)wid;
+    const int m_row = 8 * (lane >> 4) + (lane & 7), m_chunk = 2 * m_row + ((lane >> 3) & 1);      // matrix lane / 8: a' 8 (lane / 16) .., b' 8 (lane / 8 % 2) ..
+    const uint32_t turn_in = turn + 16u * (uint32_t)(m_chunk ^ ((m_chunk >> 3) & 1)), turn_out = turn + 16u * (uint32_t)(lane ^ ((lane >> 3) & 1));
+    const ReadShare share(p);
+    uint64_t rows = 0;
+    uint16_t* dst = p.out[side] + (size_t)share.first * (size_t)p.stride[side] + (head0 * kHeadDim + 8 * lane);
 #pragma unroll 1
-    for (long long u = (long long)blockIdx.x * kReadWarps + wid; u < p.units; u += (long long)gridDim.x * kReadWarps) {
-        const ReadUnit x = read_unit(p, u);
-        const uint8_t* row = reinterpret_cast<const uint8_t*>((uintptr_t)x.row);
-        F2 v[16];
-        float d0 = 0.0f, d1 = 0.0f;
-        if (x.row != 0) {
-            // quads: register pairs 2 k, 2 k + 1 are columns 8 (k + 8 (j / 2)) + 4 (j % 2) .. + 3
-            const uint8_t* codes = row + kTq4BlockBytes * (j >> 2) + 2 + 32 * ((j >> 1) & 1) + 2 * (j & 1);
-            uint32_t c[8];
+    for (int t = share.first; t < share.end; ++t, dst += p.stride[side]) {
+        const int k32 = (t - share.first) & 31;
+        if (k32 == 0) rows = read_rows_of(p, t, share.end, head0, side);
+        const uint8_t* row = reinterpret_cast<const uint8_t*>((uintptr_t)__shfl_sync(0xffffffffu, rows, k32));
+        if (row == nullptr) continue;
+        uint32_t codes[ROWS][2], scales[ROWS][2];      // fp16 bits of the scales
 #pragma unroll
-            for (int k = 0; k < 8; ++k) c[k] = *reinterpret_cast<const uint16_t*>(codes + 4 * k);
-            d0 = __half2float(*reinterpret_cast<const __half*>(row)) * 0.0625f;
-            d1 = __half2float(*reinterpret_cast<const __half*>(row + kTq4BlockBytes)) * 0.0625f;
+        for (int i = 0; i < ROWS; ++i) {
+            if (ROWS > 1 && i >= n_rows) break;
+            const uint8_t* mine = row + (2 + 8 * gid + 2 * tig);
 #pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                v[2 * k] = *reinterpret_cast<const F2*>(table + ((c[k] & 0xffu) << 7));
-                v[2 * k + 1] = *reinterpret_cast<const F2*>(table + ((c[k] >> 1) & 0x7f80u));
+            for (int h = 0; h < 2; ++h) {
+                codes[i][h] = *reinterpret_cast<const uint16_t*>(mine + kTq4BlockBytes * h);
+                scales[i][h] = *reinterpret_cast<const uint16_t*>(row + kTq4BlockBytes * h);
             }
-        } else {
-#pragma unroll
-            for (int k = 0; k < 16; ++k) v[k] = 0ull;
+            row += head_stride;
         }
-        // column bits 0 (inside a pair), 1, 3, 4, 5
 #pragma unroll
-        for (int k = 0; k < 16; ++k) v[k] = f2(f2x(v[k]) + f2y(v[k]), f2x(v[k]) - f2y(v[k]));
-        read_level(v, 1, minus_one);
-        read_level(v, 2, minus_one);
-        read_level(v, 4, minus_one);
-        read_level(v, 8, minus_one);
-        __syncwarp();      // the rows of the unit before have been read
+        for (int i = 0; i < ROWS; ++i) {
+            if (ROWS > 1 && i >= n_rows) break;
+            float u[2][4];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            *reinterpret_cast<ulonglong2*>(turn + 16 * read_quad_place(2 * (k + 8 * (j >> 1)) + (j & 1))) = make_ulonglong2(v[2 * k], v[2 * k + 1]);
-        }
-        __syncwarp();
-        // chunks: pairs 4 i .. 4 i + 3 are columns 8 (j + 8 i) .. + 7
+            for (int h = 0; h < 2; ++h) {      // the half with scale d[h]: a = 8 h + n
+                const uint2 e0 = *reinterpret_cast<const uint2*>(table + (((codes[i][h] << 7) & 0x7f80u) | copy));
+                const uint2 e1 = *reinterpret_cast<const uint2*>(table + (((codes[i][h] >> 1) & 0x7f80u) | copy));
+                float z[4];
+                read_mma_zero(z, ha[0], ha[1], ha[2], ha[3], e0.x, e1.x);
+                read_mma(z, ha[0], ha[1], ha[2], ha[3], e0.y, e1.y);
+                uint32_t v0, v1, r0, r1;
+                read_split(z[0], z[1], v0, r0);
+                read_split(z[2], z[3], v1, r1);
+                read_mma8_zero(u[h], v0, v1, hb);
+                read_mma8(u[h], r0, r1, hb);
+            }
+            const float d0 = __half2float(__ushort_as_half((unsigned short)scales[i][0])), d1 = __half2float(__ushort_as_half((unsigned short)scales[i][1]));
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            const ulonglong2 q = *reinterpret_cast<const ulonglong2*>(turn + 16 * read_quad_place(2 * (j + 8 * (k >> 1)) + (k & 1)));
-            v[2 * k] = q.x;
-            v[2 * k + 1] = q.y;
-        }
-        read_level(v, 2, minus_one);      // column bit 2
-        read_level(v, 4, minus_one);      // column bit 6
-        const F2 s0 = f2(d0, d0), s1 = f2(d1, d1), n1 = f2(-d1, -d1);
+            for (int k = 0; k < 4; ++k) u[0][k] *= d0;
+            uint32_t w[2][2];      // matrices (a' 8 n .., b' 8 m ..)
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {     // column bit 7, and the scales of the two halves
-            const F2 a = f2mul(v[k], s0), b = v[k + 8];
-            v[k] = f2fma(b, s1, a);
-            v[k + 8] = f2fma(b, n1, a);
-        }
-        if (x.row == 0) continue;
-        uint16_t* dst = p.out[x.side] + (size_t)x.tok * (size_t)p.stride[x.side] + (size_t)x.head * kHeadDim + 8 * j;
+            for (int n = 0; n < 2; ++n) {
+                const float d = n ? -d1 : d1;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            uint32_t w[4];
+                for (int m = 0; m < 2; ++m) w[n][m] = read_narrow<BF16>(__fmaf_rn(d, u[1][2 * m], u[0][2 * m]), __fmaf_rn(d, u[1][2 * m + 1], u[0][2 * m + 1]));
+            }
+            __syncwarp();      // the row before has been read
+            asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};"
+                         ::"r"(turn_in), "r"(w[0][0]), "r"(w[0][1]), "r"(w[1][0]), "r"(w[1][1]) : "memory");
+            __syncwarp();
+            uint32_t r[4];
+            asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(turn_out) : "memory");
 #pragma unroll
-            for (int k = 0; k < 4; ++k) w[k] = read_narrow<BF16>(f2x(v[4 * i + k]), f2y(v[4 * i + k])) ^ sign[4 * i + k];
-            read_store8(dst + 64 * i, p.aligned, w);
+            for (int k = 0; k < 4; ++k) r[k] ^= sign[k];
+            uint16_t* to = dst + i * kHeadDim;
+            if (p.aligned) {
+                *reinterpret_cast<uint4*>(to) = make_uint4(r[0], r[1], r[2], r[3]);
+            } else {
+#pragma unroll
+                for (int k = 0; k < 4; ++k) { to[2 * k] = (uint16_t)r[k]; to[2 * k + 1] = (uint16_t)(r[k] >> 16); }
+            }
         }
     }
 }
 
-// Rows that are not rotated.  Lane j of a row: chunks j + 8 i.
-template <bool BF16>
-__global__ void __launch_bounds__(kReadWarps * 32) kv_read_plain_kernel(const ReadParams p) {
+// Rows that are not rotated: lane l holds columns 8 l .. + 7.
+template <bool BF16, int ROWS>
+__global__ void __launch_bounds__(kReadWarps * 32) kv_read_plain_kernel(const __grid_constant__ ReadParams p) {
     grid_dependency_wait();
     grid_launch_dependents();
-    const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5, j = lane & 7;
+    const int lane = threadIdx.x & 31;
+    const int heads = p.layout.local_kv_heads, groups = (heads + ROWS - 1) / ROWS;
+    const int side = p.first + (int)blockIdx.y / groups, head0 = (int)blockIdx.y % groups * ROWS;
+    const uint64_t head_stride = side == 0 ? p.layout.k_head_stride_bytes : p.layout.v_head_stride_bytes;
+    const int format = side == 0 ? p.layout.k_format : p.layout.v_format;
+    const ReadShare share(p);
+    uint64_t rows = 0;
+    uint16_t* dst = p.out[side] + (size_t)share.first * (size_t)p.stride[side] + (head0 * kHeadDim + 8 * lane);
 #pragma unroll 1
-    for (long long u = (long long)blockIdx.x * kReadWarps + wid; u < p.units; u += (long long)gridDim.x * kReadWarps) {
-        const ReadUnit x = read_unit(p, u);
-        if (x.row == 0) continue;
-        const uint8_t* row = reinterpret_cast<const uint8_t*>((uintptr_t)x.row);
-        const int format = x.side == 0 ? p.layout.k_format : p.layout.v_format;
-        uint32_t raw[4][4];
-        float d[4];
-        if (format == WARP34_KV_FORMAT_FP8_E4M3) {
+    for (int t = share.first; t < share.end; ++t, dst += p.stride[side]) {
+        const int k32 = (t - share.first) & 31;
+        if (k32 == 0) rows = read_rows_of(p, t, share.end, head0, side);
+        const uint8_t* row = reinterpret_cast<const uint8_t*>((uintptr_t)__shfl_sync(0xffffffffu, rows, k32));
+        if (row == nullptr) continue;
+        uint32_t raw[ROWS][4];
+        float d[ROWS];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const uint32_t* src = reinterpret_cast<const uint32_t*>(row + 8 * (j + 8 * i));
-                raw[i][0] = src[0];
-                raw[i][1] = src[1];
-                d[i] = *reinterpret_cast<const float*>(row + kHeadDim + 4 * (i >> 1));
-            }
-        } else if (format == WARP34_KV_FORMAT_Q8_0) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const uint32_t* src = reinterpret_cast<const uint32_t*>(row + 68 * i + 4 + 8 * j);
-                raw[i][0] = src[0];
-                raw[i][1] = src[1];
-                d[i] = *reinterpret_cast<const float*>(row + 68 * i);
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const uint16_t* src = reinterpret_cast<const uint16_t*>(row) + 8 * (j + 8 * i);
+        for (int i = 0; i < ROWS; ++i) {
+            if (ROWS > 1 && head0 + i >= heads) break;
+            const uint8_t* r = row + (size_t)i * head_stride;
+            if (format == WARP34_KV_FORMAT_BF16) {
+                const uint16_t* src = reinterpret_cast<const uint16_t*>(r) + 8 * lane;
                 if (p.rows_aligned) {
                     const uint4 q = *reinterpret_cast<const uint4*>(src);
                     raw[i][0] = q.x; raw[i][1] = q.y; raw[i][2] = q.z; raw[i][3] = q.w;
@@ -252,11 +277,17 @@ __global__ void __launch_bounds__(kReadWarps * 32) kv_read_plain_kernel(const Re
 #pragma unroll
                     for (int k = 0; k < 4; ++k) raw[i][k] = (uint32_t)src[2 * k] | ((uint32_t)src[2 * k + 1] << 16);
                 }
+            } else {
+                const bool fp8 = format == WARP34_KV_FORMAT_FP8_E4M3;
+                const uint32_t* src = reinterpret_cast<const uint32_t*>(r + (fp8 ? 8 * lane : 68 * (lane >> 3) + 4 + 8 * (lane & 7)));
+                raw[i][0] = src[0];
+                raw[i][1] = src[1];
+                d[i] = *reinterpret_cast<const float*>(r + (fp8 ? kHeadDim + 4 * (lane >> 4) : 68 * (lane >> 3)));
             }
         }
-        uint16_t* dst = p.out[x.side] + (size_t)x.tok * (size_t)p.stride[x.side] + (size_t)x.head * kHeadDim + 8 * j;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < ROWS; ++i) {
+            if (ROWS > 1 && head0 + i >= heads) break;
             uint32_t w[4];
             if (format == WARP34_KV_FORMAT_BF16) {
 #pragma unroll
@@ -280,7 +311,13 @@ __global__ void __launch_bounds__(kReadWarps * 32) kv_read_plain_kernel(const Re
                     w[k] = read_narrow<BF16>(d[i] * a, d[i] * b);
                 }
             }
-            read_store8(dst + 64 * i, p.aligned, w);
+            uint16_t* to = dst + (size_t)i * kHeadDim;
+            if (p.aligned) {
+                *reinterpret_cast<uint4*>(to) = make_uint4(w[0], w[1], w[2], w[3]);
+            } else {
+#pragma unroll
+                for (int k = 0; k < 4; ++k) { to[2 * k] = (uint16_t)w[k]; to[2 * k + 1] = (uint16_t)(w[k] >> 16); }
+            }
         }
     }
 }
@@ -330,15 +367,23 @@ static int launch_kv_read(const warp34_exec* ex, const warp34_kv_layer_layout* l
     p.sides = (k_out != nullptr ? 1 : 0) + (v_out != nullptr ? 1 : 0);
     p.aligned = ((((uintptr_t)k_out) | ((uintptr_t)v_out)) & 15u) == 0u && (k_out == nullptr || k_row_stride % 8 == 0) && (v_out == nullptr || v_row_stride % 8 == 0);
     p.rows_aligned = (bits & 15u) == 0u;
-    p.units = (((long long)batch->total_tokens + 3) / 4) * l.local_kv_heads * p.sides;
-    const long long needed = (p.units + kReadWarps - 1) / kReadWarps;
-    const long long resident = (long long)read_sm_count() * (tq4 ? 3 : 6);
-    const unsigned blocks = (unsigned)(needed < resident ? needed : resident);
+    const int sms = read_sm_count();
+    const int cols_y = p.sides * l.local_kv_heads;      // rows of a token
+    // Four heads a warp, their loads in flight together, where that still leaves every SM several blocks.
+    const bool wide = (long long)batch->total_tokens * cols_y >= 32ll * kReadWarps * sms;
+    const int rows_y = wide ? p.sides * ((l.local_kv_heads + kReadRows - 1) / kReadRows) : cols_y;
+    if (rows_y > 65535) return (int)cudaErrorInvalidValue;
+    const long long needed = ((long long)batch->total_tokens + kReadWarps - 1) / kReadWarps;
+    const long long resident = ((long long)sms * (tq4 ? kReadTq4Blocks : 8)) / rows_y > 0 ? ((long long)sms * (tq4 ? kReadTq4Blocks : 8)) / rows_y : 1;
+    const dim3 grid((unsigned)(needed < resident ? needed : resident), (unsigned)rows_y);
+    p.tokens_per_warp = (int)(((long long)batch->total_tokens + (long long)grid.x * kReadWarps - 1) / ((long long)grid.x * kReadWarps));
     cudaStream_t st = (cudaStream_t)ex->stream;
-    if (!tq4) return launch_behind(kv_read_plain_kernel<BF16>, dim3(blocks), kReadWarps * 32, 0, st, p);
-    const int rc = (int)cudaFuncSetAttribute(kv_read_tq4_kernel<BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize, kReadTableBytes + kReadTurnBytes);
-    if (rc != 0) return rc;
-    return launch_behind(kv_read_tq4_kernel<BF16>, dim3(blocks), kReadWarps * 32, kReadTableBytes + kReadTurnBytes, st, p);
+    if (!tq4) {
+        return wide ? launch_behind(kv_read_plain_kernel<BF16, kReadRows>, grid, kReadWarps * 32, 0, st, p)
+                    : launch_behind(kv_read_plain_kernel<BF16, 1>, grid, kReadWarps * 32, 0, st, p);
+    }
+    return wide ? launch_behind(kv_read_tq4_kernel<BF16, kReadRows>, grid, kReadWarps * 32, 0, st, p)
+                : launch_behind(kv_read_tq4_kernel<BF16, 1>, grid, kReadWarps * 32, 0, st, p);
 }
 
 }  // namespace w34
