@@ -481,31 +481,39 @@ def paged_attention_scored(ex, layer, batch, q, out, num_q_heads, softcap=0.0, s
     """warp34_paged_attention_scored_f16 / _bf16 (by q's type): attention with capped scores (softcap), a penalty of slopes[head] per key of
     distance, and a range of keys [key_begin, key_end) per token (int32 [tokens]; key_end in place of causality)."""
     lib = lib or ffi.kernels()
-    dtype, n = q.dtype, batch.desc.total_tokens
-    _require(dtype in (torch.float16, torch.bfloat16) and out.dtype == dtype and q.is_contiguous() and out.is_contiguous() and
-             q.numel() >= n * num_q_heads * 256 and out.numel() >= n * num_q_heads * 256,
-             f"paged_attention_scored: contiguous fp16 or bf16 q and out of [{n}, {num_q_heads}, 256]")
+    desc, dtype = batch.desc, q.dtype
+    n = desc.total_tokens
+    if not (dtype is torch.float16 or dtype is torch.bfloat16) or out.dtype is not dtype or not q.is_contiguous() or not out.is_contiguous() or \
+            q.numel() < n * num_q_heads * 256 or out.numel() < n * num_q_heads * 256:
+        raise ValueError(f"paged_attention_scored: contiguous fp16 or bf16 q and out of [{n}, {num_q_heads}, 256]")
     c = ffi.ScoreChange(None, None, None, softcap, 0)
     if slopes is not None:
-        _require(slopes.dtype == torch.float32 and slopes.numel() == num_q_heads and slopes.is_contiguous(), f"slopes: fp32 [{num_q_heads}]")
+        _require(slopes.dtype is torch.float32 and slopes.numel() == num_q_heads and slopes.is_contiguous(), "slopes: fp32, one per query head")
         c.distance_slopes = slopes.data_ptr()
     if key_begin is not None:
-        _require(key_begin.dtype == torch.int32 and key_begin.numel() >= n and key_begin.is_contiguous(), f"key_begin: int32 [{n}]")
+        _require(key_begin.dtype is torch.int32 and key_begin.numel() >= n and key_begin.is_contiguous(), "key_begin: int32, one per token")
         c.key_begin = key_begin.data_ptr()
     if key_end is not None:
-        _require(key_end.dtype == torch.int32 and key_end.numel() >= n and key_end.is_contiguous(), f"key_end: int32 [{n}]")
+        _require(key_end.dtype is torch.int32 and key_end.numel() >= n and key_end.is_contiguous(), "key_end: int32, one per token")
         c.key_end = key_end.data_ptr()
     fn = lib.warp34_paged_attention_scored_f16 if dtype == torch.float16 else lib.warp34_paged_attention_scored_bf16
-    _check(fn(C.byref(ex.ex), C.byref(layer.layout), C.byref(batch.desc), C.byref(c), q.data_ptr(), out.data_ptr(), num_q_heads),
-           "warp34_paged_attention_scored")
+    _check(fn(ex.ex, layer.layout, desc, c, q.data_ptr(), out.data_ptr(), num_q_heads), "warp34_paged_attention_scored")
 
 
-def _head_rows(t, dtype, heads, width, what):
-    """Checks that t is [tokens, heads, width] with heads next to each other; returns its token stride."""
-    _require(t.dtype == dtype and t.dim() == 3 and t.shape[2] == width and (heads is None or t.shape[1] == heads),
-             f"{what}: expected {dtype} of shape [tokens, heads, {width}], got {t.dtype} {tuple(t.shape)}")
-    _require((t.stride(2) == 1 or t.numel() == 0) and (t.stride(1) == width or t.shape[1] <= 1), f"{what}: heads must be contiguous")
-    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1] * width)
+def _head_rows(t, dtype, n, heads, width, what):
+    """Checks that t is [n tokens, heads, width] with heads next to each other; returns its token stride."""
+    shape, stride = t.shape, t.stride()
+    if t.dtype is not dtype or len(shape) != 3 or shape[0] != n or shape[2] != width or (heads is not None and shape[1] != heads):
+        raise ValueError(f"{what}: expected {dtype} of shape [{n} tokens, heads, {width}], got {t.dtype} {tuple(shape)}")
+    if (stride[2] != 1 or (stride[1] != width and shape[1] > 1)) and t.numel() > 0:
+        raise ValueError(f"{what}: heads must be contiguous")
+    return stride[0] if n > 1 else max(stride[0], shape[1] * width)
+
+
+def _norm_weight(w, dtype, what):
+    if w.dtype is not dtype or w.numel() != 256 or not w.is_contiguous():
+        raise ValueError(f"{what}_weight: 256 contiguous values of {dtype}")
+    return w.data_ptr()
 
 
 def qk_norm_rope(ex, q, k, q_weight, k_weight, positions, inv_freq, q_out, k_out, gate_out=None, sections=None, eps=1e-6,
@@ -516,62 +524,62 @@ def qk_norm_rope(ex, q, k, q_weight, k_weight, positions, inv_freq, q_out, k_out
     heads, 256]; either may be None with its weight and output.  Rows may be slices of packed projection rows.  positions: int32
     [tokens], or [3, tokens] with the mRoPE sections; inv_freq: fp32 [rotary_dim / 2]; None: no rotation."""
     lib = lib or ffi.kernels()
-    _require(q is not None or k is not None, "qk_norm_rope: neither q nor k")
-    dtype = (q if q is not None else k).dtype
-    _require(dtype in (torch.float16, torch.bfloat16), f"qk_norm_rope: fp16 or bf16 rows, got {dtype}")
-    a = ffi.QkNormRopeArgs()
-    n = (q if q is not None else k).shape[0]
-    for name, x, w, out in (("q", q, q_weight, q_out), ("k", k, k_weight, k_out)):
-        if x is None:
-            continue
-        width = 512 if name == "q" and gate_out is not None else 256
-        stride_in, stride_out = _head_rows(x, dtype, None, width, name), _head_rows(out, dtype, x.shape[1], 256, f"{name}_out")
-        _require(x.shape[0] == n and out.shape[0] == n, f"qk_norm_rope: {name} and {name}_out of {n} tokens")
-        _require(w.dtype == dtype and w.numel() == 256 and w.is_contiguous(), f"{name}_weight: 256 contiguous values of {dtype}")
-        setattr(a, f"{name}_in", x.data_ptr())
-        setattr(a, f"{name}_out", out.data_ptr())
-        setattr(a, f"{name}_norm_w", w.data_ptr())
-        setattr(a, f"{name}_in_stride", stride_in)
-        setattr(a, f"{name}_out_stride", stride_out)
-        setattr(a, "num_q_heads" if name == "q" else "num_kv_heads", x.shape[1])
+    first = q if q is not None else k
+    _require(first is not None, "qk_norm_rope: neither q nor k")
+    dtype, n = first.dtype, first.shape[0]
+    _require(dtype is torch.float16 or dtype is torch.bfloat16, "qk_norm_rope: fp16 or bf16 rows")
+    q_in = q_to = q_w = k_in = k_to = k_w = gate_to = mask = pos = freq = None
+    hq = hkv = qs = qos = ks = kos = gs = plane = rotary = planes = s1 = s2 = 0
+    if q is not None:
+        hq = q.shape[1]
+        qs, qos = _head_rows(q, dtype, n, None, 256 if gate_out is None else 512, "q"), _head_rows(q_out, dtype, n, hq, 256, "q_out")
+        q_in, q_to, q_w = q.data_ptr(), q_out.data_ptr(), _norm_weight(q_weight, dtype, "q")
+    if k is not None:
+        hkv = k.shape[1]
+        ks, kos = _head_rows(k, dtype, n, None, 256, "k"), _head_rows(k_out, dtype, n, hkv, 256, "k_out")
+        k_in, k_to, k_w = k.data_ptr(), k_out.data_ptr(), _norm_weight(k_weight, dtype, "k")
     if gate_out is not None:
         _require(q is not None, "qk_norm_rope: a gate without queries")
-        a.gate_out_stride = _head_rows(gate_out, dtype, q.shape[1], 256, "gate_out")
-        _require(gate_out.shape[0] == n, f"qk_norm_rope: gate_out of {n} tokens")
-        a.gate_out = gate_out.data_ptr()
+        gs, gate_to = _head_rows(gate_out, dtype, n, hq, 256, "gate_out"), gate_out.data_ptr()
     if inv_freq is not None and inv_freq.numel() > 0:
-        _require(inv_freq.dtype == torch.float32 and inv_freq.is_contiguous(), "inv_freq: contiguous fp32")
-        _require(positions.dtype == torch.int32 and positions.shape[-1] == n and positions.dim() in (1, 2) and (n <= 1 or positions.stride(-1) == 1),
-                 f"positions: int32 [{n}] or [3, {n}]")
-        planes = 1 if positions.dim() == 1 else positions.shape[0]
-        _require(planes in (1, 3) and (planes == 1 or sections is not None), "positions: one plane, or three and their sections")
-        a.positions, a.inv_freq, a.rotary_dim, a.position_planes = positions.data_ptr(), inv_freq.data_ptr(), 2 * inv_freq.numel(), planes
+        _require(inv_freq.dtype is torch.float32 and inv_freq.is_contiguous(), "inv_freq: contiguous fp32")
+        shape, stride = positions.shape, positions.stride()
+        planes = 1 if len(shape) == 1 else shape[0]
+        if positions.dtype is not torch.int32 or len(shape) > 2 or shape[-1] != n or (stride[-1] != 1 and n > 1) or \
+                not (planes == 1 or (planes == 3 and sections is not None)):
+            raise ValueError(f"positions: int32 [{n}], or [3, {n}] and their sections")
+        pos, freq, rotary = positions.data_ptr(), inv_freq.data_ptr(), 2 * inv_freq.numel()
         if planes == 3:
-            a.position_plane_stride, a.mrope_s1, a.mrope_s2 = positions.stride(0), sections[1], sections[2]
+            plane, s1, s2 = stride[0], sections[1], sections[2]
     if valid_token_mask is not None:
-        _require(valid_token_mask.dtype == torch.uint8 and valid_token_mask.numel() == n and valid_token_mask.is_contiguous(),
-                 f"valid_token_mask: uint8 [{n}]")
-        a.valid_token_mask = valid_token_mask.data_ptr()
-    a.num_tokens, a.head_dim, a.rms_eps, a.weight_offset = n, 256, eps, weight_offset
-    fn = lib.warp34_qk_norm_rope_f16 if dtype == torch.float16 else lib.warp34_qk_norm_rope_bf16
-    _check(fn(C.byref(ex.ex), C.byref(a)), "warp34_qk_norm_rope")
+        _require(valid_token_mask.dtype is torch.uint8 and valid_token_mask.numel() == n and valid_token_mask.is_contiguous(),
+                 "valid_token_mask: uint8, one per token")
+        mask = valid_token_mask.data_ptr()
+    a = ffi.QkNormRopeArgs(q_in, k_in, q_to, k_to, gate_to, q_w, k_w, pos, freq, mask, qs, ks, qos, kos, gs, plane,
+                           n, hq, hkv, 256, rotary, planes, s1, s2, eps, weight_offset)
+    fn = lib.warp34_qk_norm_rope_f16 if dtype is torch.float16 else lib.warp34_qk_norm_rope_bf16
+    _check(fn(ex.ex, a), "warp34_qk_norm_rope")
 
 
 def kv_cache_read(ex, layer, batch, k_out, v_out, lib=None):
     """warp34_kv_cache_read_f16 / _bf16 (by the outputs' type): the rows of the batch's tokens read back into k_out / v_out [tokens,
     heads * 256] (either may be None)."""
     lib = lib or ffi.kernels()
-    outs = [t for t in (k_out, v_out) if t is not None]
-    _require(outs and all(t.dtype == outs[0].dtype for t in outs) and outs[0].dtype in (torch.float16, torch.bfloat16),
-             "kv_cache_read: fp16 or bf16 outputs of one type")
-    n, cols = batch.desc.total_tokens, layer.layout.local_kv_heads * layer.layout.head_dim
-    for t in outs:
-        _require(t.dim() == 2 and t.shape[0] >= n and t.shape[1] == cols and t.stride(1) == 1, f"kv_cache_read: outputs [{n}, {cols}]")
-    stride = lambda t: 0 if t is None else t.stride(0) if t.shape[0] > 1 else max(t.stride(0), cols)  # noqa: E731
-    ptr = lambda t: None if t is None else t.data_ptr()  # noqa: E731
-    fn = lib.warp34_kv_cache_read_f16 if outs[0].dtype == torch.float16 else lib.warp34_kv_cache_read_bf16
-    _check(fn(C.byref(ex.ex), C.byref(layer.layout), C.byref(batch.desc), ptr(k_out), ptr(v_out), stride(k_out), stride(v_out)),
-           "warp34_kv_cache_read")
+    desc, layout = batch.desc, layer.layout
+    n, cols = desc.total_tokens, layout.local_kv_heads * layout.head_dim
+    dtype, at = None, []
+    for t in (k_out, v_out):
+        if t is None:
+            at += (None, 0)
+            continue
+        shape, stride = t.shape, t.stride()
+        if len(shape) != 2 or shape[0] < n or shape[1] != cols or stride[1] != 1 or (dtype is not None and t.dtype is not dtype):
+            raise ValueError(f"kv_cache_read: outputs of one type, [{n}, {cols}]")
+        dtype = t.dtype
+        at += (t.data_ptr(), stride[0] if shape[0] > 1 else max(stride[0], cols))
+    _require(dtype is torch.float16 or dtype is torch.bfloat16, "kv_cache_read: fp16 or bf16 outputs")
+    fn = lib.warp34_kv_cache_read_f16 if dtype is torch.float16 else lib.warp34_kv_cache_read_bf16
+    _check(fn(ex.ex, layout, desc, at[0], at[2], at[1], at[3]), "warp34_kv_cache_read")
 
 
 def kv_page_copy(ex, layer, src_page, dst_page, rows, lib=None):
