@@ -196,8 +196,9 @@ __global__ void __launch_bounds__(kBfWarps * 32, 1) bf16kv_attention_stream_kern
         const int32_t* blocks = p.batch.block_tables + (size_t)r * p.batch.max_blocks_per_req;
         const uint8_t* k_head_base = (const uint8_t*)(uintptr_t)p.layout.k_base + (size_t)kv_head * p.layout.k_head_stride_bytes;
         const uint8_t* v_head_base = (const uint8_t*)(uintptr_t)p.layout.v_base + (size_t)kv_head * p.layout.v_head_stride_bytes;
+        auto logical = [&](int idx) { return SCORED ? pg0 + n_here - 1 - idx : pg0 + idx; };      // SCORED: the last page first, see x_stream()
         auto issue = [&](int idx) {
-            const int32_t page = block_table_page(blocks, pg0 + idx, p.batch.max_blocks_per_req, kInBf16);
+            const int32_t page = block_table_page(blocks, logical(idx), p.batch.max_blocks_per_req, kInBf16);
             const uint8_t* ks = k_head_base + (size_t)page * p.layout.k_page_stride_bytes + lane * 16;
             const uint8_t* vs = v_head_base + (size_t)page * p.layout.v_page_stride_bytes + lane * 16;
             const uint32_t dst = ring + (uint32_t)(idx % kBfStages) * kBfStageBytes + lane * 16;
@@ -215,7 +216,7 @@ __global__ void __launch_bounds__(kBfWarps * 32, 1) bf16kv_attention_stream_kern
             cp_async_wait<1>();
             __syncwarp();
             const uint32_t kt = ring + (uint32_t)(i % kBfStages) * kBfStageBytes, vt = kt + kBfTileBytes;
-            const int kv_base = (pg0 + i) << 4;
+            const int kv_base = logical(i) << 4;
             const bool full = (kv_base >= safe_lo) && (kv_base + 15 <= safe_hi);
 
             float sacc[2][4];

@@ -458,10 +458,11 @@ __global__ void __launch_bounds__(kKv8StreamWarps * 32, 1) kv8_attention_stream_
         const int32_t* blocks = p.batch.block_tables + (size_t)r * p.batch.max_blocks_per_req;
         const uint8_t* k_head_base = (const uint8_t*)(uintptr_t)p.layout.k_base + (size_t)kv_head * p.layout.k_head_stride_bytes;
         const uint8_t* v_head_base = (const uint8_t*)(uintptr_t)p.layout.v_base + (size_t)kv_head * p.layout.v_head_stride_bytes;
+        auto logical = [&](int idx) { return SCORED ? pg0 + n_here - 1 - idx : pg0 + idx; };      // SCORED: the last page first, see x_stream()
         int32_t my_page = 0, next_page = 0;
         if (!SPARSE) {
-            my_page = (lane < n_here) ? block_table_page(blocks, pg0 + lane, p.batch.max_blocks_per_req, kInKv8) : 0;
-            next_page = (32 + lane < n_here) ? block_table_page(blocks, pg0 + 32 + lane, p.batch.max_blocks_per_req, kInKv8) : 0;
+            my_page = (lane < n_here) ? block_table_page(blocks, logical(lane), p.batch.max_blocks_per_req, kInKv8) : 0;
+            next_page = (32 + lane < n_here) ? block_table_page(blocks, logical(32 + lane), p.batch.max_blocks_per_req, kInKv8) : 0;
         }
         const int32_t* sel_phys = SPARSE ? p.sel_phys + (size_t)r * p.select_k : nullptr;
         const int32_t* sel_logical = SPARSE ? p.sel_logical + (size_t)r * p.select_k : nullptr;
@@ -525,7 +526,7 @@ __global__ void __launch_bounds__(kKv8StreamWarps * 32, 1) kv8_attention_stream_
         for (int i = 0; i < n_here; ++i) {
             if (!SPARSE && (i & 31) == 0 && i > 0) {
                 const int base = i + 32;
-                const int32_t fresh = (base + lane < n_here) ? block_table_page(blocks, pg0 + base + lane, p.batch.max_blocks_per_req, kInKv8) : 0;
+                const int32_t fresh = (base + lane < n_here) ? block_table_page(blocks, logical(base + lane), p.batch.max_blocks_per_req, kInKv8) : 0;
                 if (i & 32) my_page = fresh; else next_page = fresh;
             }
             {
@@ -538,7 +539,7 @@ __global__ void __launch_bounds__(kKv8StreamWarps * 32, 1) kv8_attention_stream_
             pending &= ~(1u << s);
 
             const uint32_t st = ring + (uint32_t)s * kStage;
-            const int kv_base = (pg0 + i) << 4;
+            const int kv_base = logical(i) << 4;
             bool full = (kv_base >= safe_lo) && (kv_base + 15 <= safe_hi);
             // query-sparse: first position of the unit's four groups (0x3fffffff: nothing was copied)
             int fpos[4] = {0, 0, 0, 0};

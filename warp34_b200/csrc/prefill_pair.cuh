@@ -108,6 +108,8 @@ __device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((u
 template <int FMT> struct PpSmem {
     static constexpr bool kDirect = FMT == WARP34_KV_FORMAT_BF16;
     static constexpr int kStages = kDirect ? 8 : kPpStages;
+    static constexpr int kConsumers = kDirect ? 8 : 4;          // consumer warps: one or two threads a row
+    static constexpr int kFillers = kDirect ? 2 : 4;            // warps that fill K stages, and V stages
     static constexpr uint32_t kStage = kDirect ? kPpPart : kPpStage;
     static constexpr uint32_t kRun = kPageTokens * PpFormat<FMT>::kRow;      // one (page, head) run
     static constexpr uint32_t kRawK = kDirect ? 0u : 2u * kRun, kRawV = kDirect ? 0u : 4u * kRun;
@@ -118,8 +120,9 @@ template <int FMT> struct PpSmem {
     static constexpr uint32_t kOffRaw = kOffQLo + (PpFormat<FMT>::kRotated ? kPpQLoBytes : 0u);
     static constexpr uint32_t kOffLut = kDirect ? (uint32_t)kPpCtaRows * kPpOutStride * 4u : (kOffRaw + kPpRawStages * kRaw + 127u) & ~127u;
     static constexpr uint32_t kOffBars = kOffLut + (PpFormat<FMT>::kRotated ? kPpLutBytes : 0u);
-    static constexpr uint32_t kWords = kDirect ? 384u : 224u;      // words behind the barriers, from kOffBars
-    static constexpr uint32_t kBytes = kOffBars + kWords + 64u;
+    static constexpr uint32_t kWords = kDirect ? 448u : 224u;      // words behind the barriers, from kOffBars
+    static constexpr uint32_t kOffMax = kOffBars + kWords + 64u;      // two threads a row: [block parity][half][row] maxima
+    static constexpr uint32_t kBytes = kOffMax + (kDirect ? 2u * 2u * kPpCtaRows * 4u : 0u);
     static_assert(kOffRaw <= kOffLut, "stages end before what follows them");
     static_assert(kPpCtaRows * kPpOutStride * 4 <= (int)kOffLut, "epilogue staging must end before the table");
     static_assert(kPpCtaRows * 512 <= (int)kOffQLo, "Q' staging fits the tile stages");
@@ -129,7 +132,8 @@ template <int FMT> struct PpSmem {
     // Empty, S, Pv: one arrival per CTA from the MMA warp's commits.  Raw*: within a CTA.
     enum { FullK = 0, FullV = FullK + kStages, EmptyK = FullV + kStages, EmptyV = EmptyK + kStages, SReady = EmptyV + kStages, PReady = SReady + 2,
            Pv = PReady + 2, Drain = Pv + 2, RawKFull, RawKFree = RawKFull + kPpRawStages, RawVFull = RawKFree + kPpRawStages,
-           RawVFree = RawVFull + kPpRawStages, BarCount = RawVFree + kPpRawStages };
+           RawVFree = RawVFull + kPpRawStages, Halves = RawVFree + kPpRawStages,
+           BarCount = Halves + (kDirect ? 4 : 0) };
     static_assert((uint32_t)BarCount * 8u <= kWords, "barrier slots end before the words behind them");
 };
 
@@ -455,7 +459,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPpThreads, 1) atten
     constexpr bool DIRECT = S::kDirect;
     constexpr int kPpFullK = S::FullK, kPpFullV = S::FullV, kPpEmptyK = S::EmptyK, kPpEmptyV = S::EmptyV, kPpS = S::SReady, kPpPReady = S::PReady,
                   kPpPv = S::Pv, kPpDrain = S::Drain, kPpRawKFull = S::RawKFull, kPpRawKFree = S::RawKFree, kPpRawVFull = S::RawVFull,
-                  kPpRawVFree = S::RawVFree;
+                  kPpRawVFree = S::RawVFree, kPpHalves = S::Halves;
     static_assert(!DIRECT || SCORED, "BF16 rows: scored attention");
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
@@ -498,8 +502,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPpThreads, 1) atten
     }
     if (tid == 0) {
         for (int s = 0; s < S::kStages; ++s) {
-            mbar_init(bar(kPpFullK + s), 8u);      // four producer warps of each CTA
-            mbar_init(bar(kPpFullV + s), 8u);
+            mbar_init(bar(kPpFullK + s), 2u * S::kFillers);      // the producer warps of both CTAs
+            mbar_init(bar(kPpFullV + s), 2u * S::kFillers);
             mbar_init(bar(kPpEmptyK + s), 1u);
             mbar_init(bar(kPpEmptyV + s), 1u);
         }
@@ -507,8 +511,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPpThreads, 1) atten
         mbar_init(bar(kPpS + 1), 1u);
         mbar_init(bar(kPpPv), 1u);
         mbar_init(bar(kPpPv + 1), 1u);
-        mbar_init(bar(kPpPReady), 8u);             // four consumer warps of each CTA
-        mbar_init(bar(kPpPReady + 1), 8u);
+        mbar_init(bar(kPpPReady), 2u * S::kConsumers);       // the consumer warps of both CTAs
+        mbar_init(bar(kPpPReady + 1), 2u * S::kConsumers);
+        if (DIRECT) {
+            for (int w = 0; w < 4; ++w) mbar_init(bar(kPpHalves + w), 2u);      // the two warps of 32 rows
+        }
         mbar_init(bar(kPpDrain), 1u);
         for (int s = 0; s < kPpRawStages; ++s) {
             mbar_init(bar(kPpRawKFull + s), 1u);
@@ -848,22 +855,23 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPpThreads, 1) atten
         for (int j = max(0, kn - kPpRawStages); j < kn; ++j) (void)wait_all(bar(kPpRawKFull + j % kPpRawStages), (uint32_t)((j / kPpRawStages) & 1));
         for (int j = max(0, vn - kPpRawStages); j < vn; ++j) (void)wait_all(bar(kPpRawVFull + j % kPpRawStages), (uint32_t)((j / kPpRawStages) & 1));
         }
-    } else if (DIRECT && wid >= 4) {
+    } else if (DIRECT && wid >= 8) {
         if constexpr (DIRECT) {
-        // ======================= BF16 rows straight into the tiles: lane = key, this warp's 32 channels of the stage's 128 ========
-        const bool is_v = wid >= 8;
-        const int quarter = wid & 3;
+        // ======================= BF16 rows straight into the tiles ========================================
+        // A warp copies a page's 16 of a stage's 32 keys, two rows of 256 bytes an instruction.
+        const bool is_v = wid >= 10;
+        const int part = wid & 1, chunk = lane & 15;
         const int full = is_v ? kPpFullV : kPpFullK, empty = is_v ? kPpEmptyV : kPpEmptyK;
         const uint8_t* head = is_v ? v_head_base : k_head_base;
         const uint64_t page_stride = is_v ? p.layout.v_page_stride_bytes : p.layout.k_page_stride_bytes;
         const uint64_t token_stride = is_v ? p.layout.v_token_stride_bytes : p.layout.k_token_stride_bytes;
-        const uint32_t tile0 = (is_v ? v_t : k_t) + (uint32_t)(quarter >> 1) * 4096u + (uint32_t)lane * 128u;
+        const uint32_t tiles = (is_v ? v_t : k_t) + (uint32_t)(chunk >> 3) * 4096u;
         const uint32_t leader_full = map_to_rank(bar(full), 0u);
-        // Key of this lane in half h of block j; K: the CTA's 32 keys in both halves.  Pages are looked up a block ahead.
-        auto key_of = [&](int j, int h) { return ((kb_lo + j) << 6) + 32 * (is_v ? h : (int)rank) + lane; };
+        // First key of this warp in half h of block j; K: the CTA's 32 keys in both halves.  Its page is looked up a block ahead.
+        auto key_of = [&](int j, int h) { return ((kb_lo + j) << 6) + 32 * (is_v ? h : (int)rank) + 16 * part; };
         auto page_of = [&](int j, int h) -> int32_t {
             const int pos = key_of(j, h);
-            return j < nblocks && pos >= kv_lo && pos <= kv_hi ? block_table_page(blocks, pos >> 4, p.batch.max_blocks_per_req, kInBf16) : -1;
+            return j < nblocks && pos + 15 >= kv_lo && pos <= kv_hi ? block_table_page(blocks, pos >> 4, p.batch.max_blocks_per_req, kInBf16) : -1;
         };
         int32_t page[2] = {page_of(0, 0), page_of(0, 1)};
         constexpr int kAhead = S::kStages - 2;      // copies in flight
@@ -886,11 +894,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPpThreads, 1) atten
                 ok = wait_all(bar(empty + st), (uint32_t)((issued / S::kStages + 1) & 1));
                 if (!ok) break;
                 const int32_t id = page[h];
-                const uint8_t* src = head + (id < 0 ? 0 : (size_t)id * page_stride + (size_t)(key_of(j, h) & 15) * token_stride) +
-                                     256 * (is_v ? (int)rank : h) + 64 * quarter;
-                const uint32_t dst = tile0 + (uint32_t)st * S::kStage;
+                const int pos0 = key_of(j, h);
+                const uint8_t* src = head + (id < 0 ? 0 : (size_t)id * page_stride) + 256 * (is_v ? (int)rank : h) + 16 * chunk;
+                const uint32_t dst = tiles + (uint32_t)st * S::kStage;
 #pragma unroll
-                for (int c = 0; c < 4; ++c) pp_copy16(dst + (uint32_t)(((4 * (quarter & 1) + c) ^ (lane & 7)) << 4), src + 16 * c, id >= 0);
+                for (int i = 0; i < 8; ++i) {
+                    const int key = 2 * i + (lane >> 4);
+                    const bool there = id >= 0 && pos0 + key >= kv_lo && pos0 + key <= kv_hi;      // others may hold never-written bytes: zeros
+                    pp_copy16(dst + (uint32_t)(16 * part + key) * 128u + (uint32_t)(((chunk & 7) ^ (key & 7)) << 4),
+                              src + (there ? (size_t)key * token_stride : 0), there);
+                }
                 asm volatile("cp.async.commit_group;" ::: "memory");
                 ++issued;
                 if (issued > kAhead) {
@@ -905,7 +918,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPpThreads, 1) atten
         asm volatile("cp.async.wait_group 0;" ::: "memory");      // (after an abort as well: nothing is in flight when the CTA leaves)
         while (told < issued) tell();
         }
-    } else if (wid >= 4) {
+    } else if (!DIRECT && wid >= 4) {
         if constexpr (!DIRECT) {
         // ======================= producers: lane = key, this warp's 32 channels of the stage's 128 ========
         const bool is_v = wid >= 8;
@@ -1036,14 +1049,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPpThreads, 1) atten
         }
     } else {
         // ======================= consumers: softmax, P, rescale =========================================
-        const int trow = row0 + tid;
+        // DIRECT: two threads a row, of warps w and w + 4, each with one half of a block's keys (one thread a row: 4.2 instead of 3.8 ms for 8 x 2048 tokens after 8192, bound
+        // by what a single warp per scheduler issues).
+        const int half = DIRECT ? wid >> 2 : 0, crow = tid & (kPpCtaRows - 1);
+        const int trow = row0 + crow;
         const int q_off = tok0 + trow / p.gqa;
         const bool row_ok = trow < rows_used &&
                             (p.batch.valid_token_mask == nullptr || p.batch.valid_token_mask[g.q_start + q_off] != 0);
         const int rmax = row_ok ? row_last_key<SCORED>(p.batch, p.sc, g, q_off) : -1;
         const int rmin = row_ok ? row_first_key<SCORED>(p.batch, p.sc, g, q_off) : 0x7fffffff;
         const float slope = SCORED && row_ok ? row_slope(p.sc, kv_head * p.gqa + trow % p.gqa) : 0.0f;
-        const uint32_t lane_base = (uint32_t)(32 * wid) << 16;
+        const uint32_t lane_base = (uint32_t)(32 * (wid & 3)) << 16;
         const uint32_t t_o = tmem + lane_base + kPpColO, t_s = tmem + lane_base + kPpColS;
         const uint32_t leader_pready = map_to_rank(bar(kPpPReady), 0u);
         const float factor = ROT ? power_of_two(ek) : 1.0f;
@@ -1077,7 +1093,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPpThreads, 1) atten
                 if (SCORED && !again) {
                     const float away = (float)(g.ctx_before + q_off - (kbase + 32 * c));
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) sv[i] = changed_score(p.sc, sv[i] * (ROT ? factor : p.score_scale), slope, away - (float)i);
+                    for (int i = 0; i < 32; ++i) sv[i] *= ROT ? factor : p.score_scale;
+                    change_scores(p.sc, sv, slope, [&](int i) { return away - (float)i; });
                 }
                 if (!all_seen && !(SCORED && again)) {
 #pragma unroll
@@ -1095,15 +1112,25 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPpThreads, 1) atten
             };
             // TQ4 reads them twice (maximum, then weights): holding all 64 spills there (92 bytes a thread, five ragged
             // prompts 270 us instead of 245), while the 8-bit builds have room and the second read costs them 10 %.
+            constexpr int PARTS = DIRECT ? 1 : 2;      // 32-key parts of the block that this thread has
             float sv[2][32];
             float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};     // four independent chains
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                scores(c, sv[ROT ? 0 : c]);
+            for (int c = 0; c < PARTS; ++c) {
+                scores(c + half, sv[ROT ? 0 : c]);
 #pragma unroll
                 for (int i = 0; i < 32; ++i) mx4[i & 3] = fmaxf(mx4[i & 3], sv[ROT ? 0 : c][i]);
             }
-            const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * (SCORED ? 1.0f : ROT ? factor : p.score_scale);
+            float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * (SCORED ? 1.0f : ROT ? factor : p.score_scale);
+            if constexpr (DIRECT) {      // the row's other half: both threads go on with the same maximum
+                float* maxima = reinterpret_cast<float*>(gen + S::kOffMax) + (j & 1) * (2 * kPpCtaRows) + crow;
+                maxima[half * kPpCtaRows] = mx;
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar(kPpHalves + (wid & 3)));
+                if (!wait_all(bar(kPpHalves + (wid & 3)), (uint32_t)(j & 1))) { *abort_flag = 1u; break; }
+                tc_fence_after();
+                mx = fmaxf(mx, maxima[(half ^ 1) * kPpCtaRows]);
+            }
             // the reference maximum moves only when the true maximum ran ahead by more than the threshold
             const bool need = mx > m_ref + kPpRescaleThreshold;
             float alpha = 1.0f;
@@ -1116,7 +1143,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPpThreads, 1) atten
                 if (!wait_all(bar(kPpPv + ((j - 1) & 1)), (uint32_t)(((j - 1) >> 1) & 1))) { *abort_flag = 1u; break; }
                 tc_fence_after();
 #pragma unroll 1
-                for (int c = 0; c < 16; ++c) {
+                for (int c = DIRECT ? 8 * half : 0; c < (DIRECT ? 8 * half + 8 : 16); ++c) {
                     uint32_t o[16];
                     tc_ld16(o, t_o + 16u * c);
                     tc_wait_ld();
@@ -1128,7 +1155,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPpThreads, 1) atten
             float ls4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
             const float m_use = ((m_ref < -1e29f) ? 0.0f : m_ref) - kPpShift;     // nothing visible yet: every P is 0
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
+            for (int c = 0; c < PARTS; ++c) {
                 uint32_t hi[16], lo[16];
                 if (ROT) scores(c, sv[0], true);
 #pragma unroll
@@ -1143,8 +1170,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPpThreads, 1) atten
                     lo[i] = pp_pack<FMT>(pa - hf.x, pb - hf.y);
                 }
                 // P takes the place of the scores it came from: value in columns 32 c .. + 15, residual in the next 16
-                tc_st16(t_sj + 32u * c, hi);
-                tc_st16(t_sj + 32u * c + 16u, lo);
+                tc_st16(t_sj + 32u * (c + half), hi);
+                tc_st16(t_sj + 32u * (c + half) + 16u, lo);
             }
             tc_wait_st();
             l_run = l_run * alpha + ((ls4[0] + ls4[1]) + (ls4[2] + ls4[3]));
@@ -1171,12 +1198,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPpThreads, 1) atten
     }
     const bool aborted = *abort_flag != 0u;
     float* stage = reinterpret_cast<float*>(gen);
-    if (wid < 4 && !aborted) {
-        float* mine = stage + tid * kPpOutStride;
+    if (wid < S::kConsumers && !aborted) {
+        const int half = DIRECT ? wid >> 2 : 0;      // DIRECT: each of the row's threads has half of its columns
+        float* mine = stage + (tid & (kPpCtaRows - 1)) * kPpOutStride;
         if (nblocks > 0) {
-            const uint32_t t_o = tmem + ((uint32_t)(32 * wid) << 16) + kPpColO;
+            const uint32_t t_o = tmem + ((uint32_t)(32 * (wid & 3)) << 16) + kPpColO;
 #pragma unroll 1
-            for (int c = 0; c < 8; ++c) {
+            for (int c = DIRECT ? 4 * half : 0; c < (DIRECT ? 4 * half + 4 : 8); ++c) {
                 uint32_t o[32];
                 tc_ld32(o, t_o + 32u * c);
                 tc_wait_ld();
@@ -1186,8 +1214,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPpThreads, 1) atten
                 }
             }
         }
-        mine[256] = l_run;
-        mine[257] = m_ref;
+        mine[DIRECT && half == 1 ? 258 : 256] = l_run;
+        if (half == 0) mine[257] = m_ref;
     }
     tc_fence_before();
     __syncthreads();
@@ -1202,7 +1230,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPpThreads, 1) atten
                 const int q_head = kv_head * p.gqa + trow % p.gqa;
                 if (p.batch.valid_token_mask != nullptr && p.batch.valid_token_mask[q_start + q_off] == 0) continue;
                 const float* src = stage + row * kPpOutStride;
-                float l = src[256], m = src[257];
+                float l = DIRECT ? src[256] + src[258] : src[256], m = src[257];
                 float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
                 if (!fits) {
                     if constexpr (SCORED) {      // (the mass and rows of the other splits carry 2^kPpShift)
@@ -1248,7 +1276,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPpThreads, 1) atten
                 const bool ok = trow < rows && (p.batch.valid_token_mask == nullptr || p.batch.valid_token_mask[q_start + q_off] != 0);
                 const bool gated = ok && p.og.mode != 0 && p.og.gate != nullptr;
                 const uint32_t at = smem_u32(smem_raw) + (uint32_t)row * (4u * kPpOutStride);
-                const float l = __uint_as_float(lds32(at + 1024u));
+                const float l = DIRECT ? __uint_as_float(lds32(at + 1024u)) + __uint_as_float(lds32(at + 1032u)) : __uint_as_float(lds32(at + 1024u));
                 float inv = l > 0.0f ? 1.0f / (ROT ? l * (kPpLutScale * 16.0f) : l) : 0.0f;
                 const bool keys = SCORED ? l != 0.0f : PpFormat<FMT>::has_keys(l);
                 if (v_exp != 0) inv *= power_of_two(v_exp);

@@ -65,7 +65,7 @@ __device__ __forceinline__ unsigned long long turns_of(float inv_freq) {
     return __double2ull_rz((x - floor(x)) * 18446744073709551616.0);
 }
 
-// Block: one token, kQkWarps * ROWS of its head rows (blockIdx.y counts them).
+// Block: one token, (warps of the block) * ROWS of its head rows (blockIdx.y counts them).
 template <bool BF16, int ROWS>
 __global__ void __launch_bounds__(kQkWarps * 32) qk_norm_rope_kernel(const QkParams p) {
     __shared__ __align__(16) float s_cos[kHeadDim / 2], s_sin[kHeadDim / 2];
@@ -75,14 +75,14 @@ __global__ void __launch_bounds__(kQkWarps * 32) qk_norm_rope_kernel(const QkPar
     const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
     const size_t tok = blockIdx.x;
     if (a.valid_token_mask != nullptr && a.valid_token_mask[tok] == 0) return;      // block-uniform
-    const int row0 = (int)blockIdx.y * (kQkWarps * ROWS) + wid;
+    const int warps = (int)(blockDim.x >> 5), row0 = (int)blockIdx.y * (warps * ROWS) + wid;
     const bool gated = a.gate_out != nullptr;
     const int q_width = gated ? 2 * kHeadDim : kHeadDim;
 
     uint32_t x[ROWS][4], gate[ROWS][4];
 #pragma unroll
     for (int i = 0; i < ROWS; ++i) {
-        const int row = row0 + kQkWarps * i;
+        const int row = row0 + warps * i;
         if (row < a.num_q_heads) {
             const uint16_t* src = static_cast<const uint16_t*>(a.q_in) + tok * (size_t)a.q_in_stride + (size_t)row * q_width + 8 * lane;
             qk_load8(src, p.aligned, x[i]);
@@ -92,8 +92,7 @@ __global__ void __launch_bounds__(kQkWarps * 32) qk_norm_rope_kernel(const QkPar
         }
     }
     const int half = a.rotary_dim >> 1;
-    if ((int)threadIdx.x < half) {
-        const int i = threadIdx.x;
+    for (int i = threadIdx.x; i < half; i += (int)blockDim.x) {
         int plane = 0;
         if (a.position_planes == 3) {
             if (i % 3 == 1 && i < 3 * a.mrope_s1) plane = 1;
@@ -128,7 +127,7 @@ __global__ void __launch_bounds__(kQkWarps * 32) qk_norm_rope_kernel(const QkPar
     }
 #pragma unroll
     for (int i = 0; i < ROWS; ++i) {
-        const int row = row0 + kQkWarps * i;
+        const int row = row0 + warps * i;
         if (row >= p.rows) break;      // warp-uniform
         const bool is_q = row < a.num_q_heads;
         float v[8], ss = 0.0f;
@@ -211,10 +210,12 @@ static int launch_qk_norm_rope(const warp34_exec* ex, const warp34_qk_norm_rope_
     cudaStream_t st = (cudaStream_t)ex->stream;
     // Four rows a warp share the token's angles; few tokens take a row a warp, so that more SMs work on each.
     const bool wide = (long long)a.num_tokens * rows >= 148ll * 8 * kQkWarps;
-    const unsigned per = (wide ? 4u : 1u) * kQkWarps;
-    const dim3 grid((unsigned)a.num_tokens, ((unsigned)rows + per - 1) / per);
-    return wide ? launch_behind(qk_norm_rope_kernel<BF16, 4>, grid, kQkWarps * 32, 0, st, p)
-                : launch_behind(qk_norm_rope_kernel<BF16, 1>, grid, kQkWarps * 32, 0, st, p);
+    // As many warps as the token's rows fill: 28 rows take seven.
+    const unsigned each = wide ? 4u : 1u, need = ((unsigned)rows + each - 1) / each, blocks = (need + kQkWarps - 1) / kQkWarps;
+    const unsigned warps = (need + blocks - 1) / blocks;
+    const dim3 grid((unsigned)a.num_tokens, blocks);
+    return wide ? launch_behind(qk_norm_rope_kernel<BF16, 4>, grid, warps * 32, 0, st, p)
+                : launch_behind(qk_norm_rope_kernel<BF16, 1>, grid, warps * 32, 0, st, p);
 }
 
 }  // namespace w34

@@ -89,7 +89,9 @@ __device__ __forceinline__ void scored_row_keys(const ScoredRow& p, int req, int
             float d = 0.0f;
 #pragma unroll
             for (int i = 0; i < 8; ++i) d = __fmaf_rn(q[i], x[i], d);
-            s[k] = changed_score(*p.sc, warp_sum(d) * scale, slope, (float)(q_pos - pos));
+            s[k] = warp_sum(d) * scale;
+            if (p.sc->cap != 0.0f) s[k] = capped_score(*p.sc, s[k]);
+            s[k] = __fmaf_rn(-slope, (float)abs(q_pos - pos), s[k]);
         }
 #pragma unroll
         for (int k = 0; k < 2; ++k) {

@@ -149,7 +149,11 @@ __device__ __forceinline__ void x_stream(const StreamParams& p, XWarp& x, int r,
     const int32_t* blocks = p.batch.block_tables + (size_t)r * p.batch.max_blocks_per_req;
     const uint8_t* k_head_base = (const uint8_t*)(uintptr_t)p.layout.k_base + (size_t)kv_head * p.layout.k_head_stride_bytes;
     const uint8_t* v_head_base = (const uint8_t*)(uintptr_t)p.layout.v_base + (size_t)kv_head * p.layout.v_head_stride_bytes;
-    auto page_of = [&](int idx) { return (idx < n_here) ? block_table_page(blocks, pg0 + idx, p.batch.max_blocks_per_req, kInStream) : 0; };
+    // SCORED: the last page first.  With a penalty on distance the newest keys hold most of the mass: met last, every page would hold most of the
+    // mass so far, the maximum would grow with each and each would take the pass over the V residuals (634 instead of 537 us for 64 sequences
+    // of 8192 to 32768).
+    auto logical = [&](int idx) { return SCORED ? pg0 + n_here - 1 - idx : pg0 + idx; };
+    auto page_of = [&](int idx) { return (idx < n_here) ? block_table_page(blocks, logical(idx), p.batch.max_blocks_per_req, kInStream) : 0; };
     int32_t my_page = 0, next_page = 0;     // page ids of units [64 c, 64 c + 32) and [64 c + 32, 64 c + 64)
     if (!SPARSE) {
         my_page = page_of(lane);
@@ -312,7 +316,7 @@ __device__ __forceinline__ void x_stream(const StreamParams& p, XWarp& x, int r,
 #pragma unroll
                 for (int c = 0; c < 4; ++c) pr[y][c] += __shfl_xor_sync(0xffffffffu, pr[y][c], 2);
             }
-            const int kv_base = (pg0 + 2 * st + y) << 4;
+            const int kv_base = logical(2 * st + y) << 4;
             if (SCORED) {
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
