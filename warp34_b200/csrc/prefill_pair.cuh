@@ -104,26 +104,31 @@ template <int FMT> struct PpScales {
 };
 __device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
 
-// BF16 rows are operands as they are: no residual parts, no raw stages (the producers copy rows straight into the tiles), more stages.
+// BF16 rows are operands as they are: no residual parts and no raw stages (the producers copy rows straight into the tiles).  That leaves
+// room for the query in shared memory, and its columns of tensor memory for blocks of 128 keys, over which the waits and exchanges of a block
+// are spread (64 keys with the query in tensor memory: 3.3 ms for 8 x 2048 tokens after 8192, 128 2.8).
 template <int FMT> struct PpSmem {
     static constexpr bool kDirect = FMT == WARP34_KV_FORMAT_BF16;
-    static constexpr int kStages = kDirect ? 8 : kPpStages;
+    static constexpr int kStages = kDirect ? 4 : kPpStages;
+    static constexpr int kKeyBits = kDirect ? 7 : 6;            // keys of a block: 128 or kPpKeys
+    static constexpr int kKeys = 1 << kKeyBits, kStageKeys = kKeys / 2;      // half of a block's keys (K: the CTA's, V: of either CTA) in a stage
     static constexpr int kConsumers = kDirect ? 8 : 4;          // consumer warps: one or two threads a row
     static constexpr int kFillers = kDirect ? 2 : 4;            // warps that fill K stages, and V stages
-    static constexpr uint32_t kStage = kDirect ? kPpPart : kPpStage;
+    static constexpr uint32_t kBlock = (uint32_t)kStageKeys * 128u;          // 64 channels of a stage's keys
+    static constexpr uint32_t kStage = (kDirect ? 2u : 4u) * kBlock;
     static constexpr uint32_t kRun = kPageTokens * PpFormat<FMT>::kRow;      // one (page, head) run
     static constexpr uint32_t kRawK = kDirect ? 0u : 2u * kRun, kRawV = kDirect ? 0u : 4u * kRun;
     static constexpr uint32_t kRaw = kRawK + kRawV;
     static constexpr uint32_t kOffK = 0;
     static constexpr uint32_t kOffV = kOffK + kStages * kStage;
     static constexpr uint32_t kOffQLo = kOffV + kStages * kStage;
-    static constexpr uint32_t kOffRaw = kOffQLo + (PpFormat<FMT>::kRotated ? kPpQLoBytes : 0u);
-    static constexpr uint32_t kOffLut = kDirect ? (uint32_t)kPpCtaRows * kPpOutStride * 4u : (kOffRaw + kPpRawStages * kRaw + 127u) & ~127u;
+    static constexpr uint32_t kOffRaw = kOffQLo + (PpFormat<FMT>::kRotated || kDirect ? kPpQLoBytes : 0u);      // (BF16: the query itself)
+    static constexpr uint32_t kOffLut = (kOffRaw + kPpRawStages * kRaw + 127u) & ~127u;
     static constexpr uint32_t kOffBars = kOffLut + (PpFormat<FMT>::kRotated ? kPpLutBytes : 0u);
     static constexpr uint32_t kWords = kDirect ? 448u : 224u;      // words behind the barriers, from kOffBars
     static constexpr uint32_t kOffMax = kOffBars + kWords + 64u;      // two threads a row: [block parity][half][row] maxima
     static constexpr uint32_t kBytes = kOffMax + (kDirect ? 2u * 2u * kPpCtaRows * 4u : 0u);
-    static_assert(kOffRaw <= kOffLut, "stages end before what follows them");
+    static_assert(kDirect || (kStage == kPpStage && kKeys == kPpKeys), "the other formats' layout");
     static_assert(kPpCtaRows * kPpOutStride * 4 <= (int)kOffLut, "epilogue staging must end before the table");
     static_assert(kPpCtaRows * 512 <= (int)kOffQLo, "Q' staging fits the tile stages");
     static_assert(!PpFormat<FMT>::kRotated || (kPpCtaRows / 4 + kPpWarps) * 2048 <= (int)kOffQLo, "so do the rows that change lanes behind it");
@@ -457,6 +462,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPpThreads, 1) atten
     constexpr bool ROT = PpFormat<FMT>::kRotated;
     constexpr uint32_t ROW = PpFormat<FMT>::kRow;
     constexpr bool DIRECT = S::kDirect;
+    constexpr int KB = S::kKeyBits;
     constexpr int kPpFullK = S::FullK, kPpFullV = S::FullV, kPpEmptyK = S::EmptyK, kPpEmptyV = S::EmptyV, kPpS = S::SReady, kPpPReady = S::PReady,
                   kPpPv = S::Pv, kPpDrain = S::Drain, kPpRawKFull = S::RawKFull, kPpRawKFree = S::RawKFree, kPpRawVFull = S::RawVFull,
                   kPpRawVFree = S::RawVFree, kPpHalves = S::Halves;
@@ -593,7 +599,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPpThreads, 1) atten
     }
     const bool any_keys = kv_hi >= kv_lo;
     const int pg_lo = any_keys ? (kv_lo >> 4) : 0, pg_hi = any_keys ? (kv_hi >> 4) : -1;
-    const int all_lo = any_keys ? (kv_lo >> 6) : 0, all = any_keys ? ((kv_hi >> 6) - all_lo + 1) : 0;
+    const int all_lo = any_keys ? (kv_lo >> KB) : 0, all = any_keys ? ((kv_hi >> KB) - all_lo + 1) : 0;
     const int kb_lo = all_lo + (int)((long long)all * blockIdx.z / p.splits);     // this split's key blocks
     const int nblocks = all_lo + (int)((long long)all * (blockIdx.z + 1) / p.splits) - kb_lo;
 
@@ -689,6 +695,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPpThreads, 1) atten
                     widen8(raw_q[i], p.io_bf16, x);
 #pragma unroll
                     for (int e = 0; e < 8; ++e) x[e] *= p.q_scale;
+                    if (DIRECT) {      // the operand tile, swizzled
+                        sts128(qlo_t + (uint32_t)i * (kPpCtaRows * 128u) + (uint32_t)row * 128u + (uint32_t)((j ^ (row & 7)) << 4), pp_pack<FMT>(x[0], x[1]),
+                               pp_pack<FMT>(x[2], x[3]), pp_pack<FMT>(x[4], x[5]), pp_pack<FMT>(x[6], x[7]));
+                        continue;
+                    }
                     sts128(q_stage + (uint32_t)row * 512u + (q_chunk_place<ROT>((uint32_t)(j + 8 * i), (uint32_t)row) << 4), pp_pack<FMT>(x[0], x[1]),
                            pp_pack<FMT>(x[2], x[3]), pp_pack<FMT>(x[4], x[5]), pp_pack<FMT>(x[6], x[7]));
                 }
@@ -736,12 +747,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPpThreads, 1) atten
         }
         if (lane == 0) { exponents[0] = ek; exponents[1] = ev; place[0] = req; place[1] = kb_lo; place[2] = tok0; place[3] = rows_used; place[4] = g.q_start; }
     }
-    if (ROT) fence_proxy_async();     // the residual tile is read by the tensor core
+    if (ROT || DIRECT) fence_proxy_async();     // the residual (BF16: the query's) tile is read by the tensor core
     tc_fence_before();
     __syncthreads();                  // staging is written
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
-    if (wid < 4) {
+    if (!DIRECT && wid < 4) {
         const uint32_t t_q = tmem + ((uint32_t)(32 * wid) << 16) + kPpColQ;
 #pragma unroll 1
         for (int c4 = 0; c4 < 4; ++c4) {
@@ -770,17 +781,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPpThreads, 1) atten
         // which PV(j - 2), issued before it, has read.
         if (rank == 0 && elect_one()) {
             constexpr uint32_t kTypes = DIRECT ? (1u << 7) | (1u << 10) : 0u;      // bf16 operands
-            constexpr uint32_t kIdescQk = tc_idesc(kPpRows, kPpKeys, 0) | kTypes;
+            constexpr uint32_t kIdescQk = tc_idesc(kPpRows, S::kKeys, 0) | kTypes;
             constexpr uint32_t kIdescPv = tc_idesc(kPpRows, kHeadDim, 1) | kTypes;
             const uint64_t desc_k = tc_smem_desc(k_t, 16u, 1024u);
-            const uint64_t desc_v = tc_smem_desc(v_t, 4096u, 1024u);
+            const uint64_t desc_v = tc_smem_desc(v_t, S::kBlock, 1024u);
             const uint64_t desc_q = tc_smem_desc(qlo_t, 16u, 1024u);
             uint32_t kst = 0, kph = 0, vst = 0, vph = 0;
             bool ok = true;
 #pragma unroll 1
             for (int j = 0; j <= nblocks && ok && *abort_flag == 0u; ++j) {
                 if (j < nblocks) {
-                    const uint32_t d = tmem + kPpColS + 64u * (uint32_t)(j & 1);
+                    const uint32_t d = tmem + kPpColS + (uint32_t)S::kKeys * (uint32_t)(j & 1);
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
                         ok = ok && mbar_wait(bar(kPpFullK + (int)kst), kph);
@@ -789,10 +800,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPpThreads, 1) atten
                         const uint64_t b0 = desc_k + (uint64_t)(kst * (S::kStage / 16));
 #pragma unroll
                         for (int ks = 0; ks < 8; ++ks) {
-                            const uint64_t b = b0 + (uint64_t)((ks >> 2) * (4096 / 16) + 2 * (ks & 3));
+                            const uint64_t b = b0 + (uint64_t)((ks >> 2) * (S::kBlock / 16) + 2 * (ks & 3));
                             const uint32_t a = tmem + kPpColQ + 64u * (uint32_t)h + 8u * (uint32_t)ks;
+                            if constexpr (DIRECT) {
+                                tc2_mma_f16(d, desc_q + (uint64_t)((2 * h + (ks >> 2)) * (kPpCtaRows * 128 / 16) + 2 * (ks & 3)), b, kIdescQk, (h || ks) ? 1u : 0u);
+                                continue;
+                            }
                             tc2_mma_f16_ts(d, a, b, kIdescQk, (h || ks) ? 1u : 0u);
-                            if (!DIRECT) tc2_mma_f16_ts(d, a, b + kPpPart / 16, kIdescQk, 1u);
+                            tc2_mma_f16_ts(d, a, b + kPpPart / 16, kIdescQk, 1u);
                             if (ROT) {
                                 tc2_mma_f16(d, desc_q + (uint64_t)((2 * h + (ks >> 2)) * (kPpCtaRows * 128 / 16) + 2 * (ks & 3)), b,
                                             kIdescQk, 1u);
@@ -806,7 +821,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPpThreads, 1) atten
                 if (j > 0 && ok) {
                     const int i = j - 1;
                     ok = mbar_wait(bar(kPpPReady + (i & 1)), (uint32_t)((i >> 1) & 1));
-                    const uint32_t a0 = tmem + kPpColS + 64u * (uint32_t)(i & 1);
+                    const uint32_t a0 = tmem + kPpColS + (uint32_t)S::kKeys * (uint32_t)(i & 1);
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
                         ok = ok && mbar_wait(bar(kPpFullV + (int)vst), vph);
@@ -814,9 +829,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPpThreads, 1) atten
                         tc_fence_after();
                         const uint64_t b0 = desc_v + (uint64_t)(vst * (S::kStage / 16));
 #pragma unroll
-                        for (int ks = 0; ks < 2; ++ks) {
+                        for (int ks = 0; ks < S::kStageKeys / 16; ++ks) {      // 16 keys: columns 32 (key / 32) + 8 (key / 16 % 2) and 16 further
                             const uint64_t b = b0 + (uint64_t)((2048 / 16) * ks);
-                            const uint32_t a = a0 + 32u * (uint32_t)h + 8u * (uint32_t)ks;
+                            const uint32_t a = a0 + (uint32_t)(S::kStageKeys * h) + 32u * (uint32_t)(ks >> 1) + 8u * (uint32_t)(ks & 1);
                             tc2_mma_f16_ts(tmem + kPpColO, a, b, kIdescPv, (i > 0 || h > 0 || ks > 0) ? 1u : 0u);
                             tc2_mma_f16_ts(tmem + kPpColO, a + 16u, b, kIdescPv, 1u);
                             if (!DIRECT) tc2_mma_f16_ts(tmem + kPpColO, a, b + kPpPart / 16, kIdescPv, 1u);
@@ -858,22 +873,22 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPpThreads, 1) atten
     } else if (DIRECT && wid >= 8) {
         if constexpr (DIRECT) {
         // ======================= BF16 rows straight into the tiles ========================================
-        // A warp copies a page's 16 of a stage's 32 keys, two rows of 256 bytes an instruction.
+        // A warp copies 32 of a stage's 64 keys, two pages, two rows of 256 bytes an instruction.
         const bool is_v = wid >= 10;
         const int part = wid & 1, chunk = lane & 15;
         const int full = is_v ? kPpFullV : kPpFullK, empty = is_v ? kPpEmptyV : kPpEmptyK;
         const uint8_t* head = is_v ? v_head_base : k_head_base;
         const uint64_t page_stride = is_v ? p.layout.v_page_stride_bytes : p.layout.k_page_stride_bytes;
         const uint64_t token_stride = is_v ? p.layout.v_token_stride_bytes : p.layout.k_token_stride_bytes;
-        const uint32_t tiles = (is_v ? v_t : k_t) + (uint32_t)(chunk >> 3) * 4096u;
+        const uint32_t tiles = (is_v ? v_t : k_t) + (uint32_t)(chunk >> 3) * S::kBlock;
         const uint32_t leader_full = map_to_rank(bar(full), 0u);
-        // First key of this warp in half h of block j; K: the CTA's 32 keys in both halves.  Its page is looked up a block ahead.
-        auto key_of = [&](int j, int h) { return ((kb_lo + j) << 6) + 32 * (is_v ? h : (int)rank) + 16 * part; };
-        auto page_of = [&](int j, int h) -> int32_t {
-            const int pos = key_of(j, h);
+        // First key of this warp in half h of block j; K: the CTA's 64 keys in both halves.  Pages are looked up a block ahead.
+        auto key_of = [&](int j, int h) { return ((kb_lo + j) << KB) + S::kStageKeys * (is_v ? h : (int)rank) + 32 * part; };
+        auto page_of = [&](int j, int h, int y) -> int32_t {
+            const int pos = key_of(j, h) + 16 * y;
             return j < nblocks && pos + 15 >= kv_lo && pos <= kv_hi ? block_table_page(blocks, pos >> 4, p.batch.max_blocks_per_req, kInBf16) : -1;
         };
-        int32_t page[2] = {page_of(0, 0), page_of(0, 1)};
+        int32_t page[2][2] = {{page_of(0, 0, 0), page_of(0, 0, 1)}, {page_of(0, 1, 0), page_of(0, 1, 1)}};
         constexpr int kAhead = S::kStages - 2;      // copies in flight
         int issued = 0, told = 0;
         auto tell = [&]() {      // the oldest stage that is not known to the MMA warp: this thread's copies into it have landed
@@ -885,7 +900,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPpThreads, 1) atten
 #pragma unroll 1
         for (int j = 0; j < nblocks; ++j) {
             if (aborted_any()) break;
-            const int32_t next[2] = {page_of(j + 1, 0), page_of(j + 1, 1)};
+            const int32_t next[2][2] = {{page_of(j + 1, 0, 0), page_of(j + 1, 0, 1)}, {page_of(j + 1, 1, 0), page_of(j + 1, 1, 1)}};
             bool ok = true;
 #pragma unroll 1
             for (int h = 0; h < 2; ++h) {
@@ -893,16 +908,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPpThreads, 1) atten
                 // parity 1: the first pass over the ring does not wait
                 ok = wait_all(bar(empty + st), (uint32_t)((issued / S::kStages + 1) & 1));
                 if (!ok) break;
-                const int32_t id = page[h];
                 const int pos0 = key_of(j, h);
-                const uint8_t* src = head + (id < 0 ? 0 : (size_t)id * page_stride) + 256 * (is_v ? (int)rank : h) + 16 * chunk;
-                const uint32_t dst = tiles + (uint32_t)st * S::kStage;
+                const uint32_t dst = tiles + (uint32_t)st * S::kStage + (uint32_t)(32 * part) * 128u;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const int key = 2 * i + (lane >> 4);
-                    const bool there = id >= 0 && pos0 + key >= kv_lo && pos0 + key <= kv_hi;      // others may hold never-written bytes: zeros
-                    pp_copy16(dst + (uint32_t)(16 * part + key) * 128u + (uint32_t)(((chunk & 7) ^ (key & 7)) << 4),
-                              src + (there ? (size_t)key * token_stride : 0), there);
+                for (int y = 0; y < 2; ++y) {
+                    const int32_t id = h == 0 ? page[0][y] : page[1][y];
+                    const uint8_t* src = head + (id < 0 ? 0 : (size_t)id * page_stride) + 256 * (is_v ? (int)rank : h) + 16 * chunk;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const int key = 2 * i + (lane >> 4), pos = pos0 + 16 * y + key;
+                        const bool there = id >= 0 && pos >= kv_lo && pos <= kv_hi;      // others may hold never-written bytes: zeros
+                        pp_copy16(dst + (uint32_t)(16 * y + key) * 128u + (uint32_t)(((chunk & 7) ^ (key & 7)) << 4), src + (there ? (size_t)key * token_stride : 0), there);
+                    }
                 }
                 asm volatile("cp.async.commit_group;" ::: "memory");
                 ++issued;
@@ -912,8 +929,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPpThreads, 1) atten
                 }
             }
             if (!ok) { *abort_flag = 1u; break; }
-            page[0] = next[0];
-            page[1] = next[1];
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {
+                page[0][y] = next[0][y];
+                page[1][y] = next[1][y];
+            }
         }
         asm volatile("cp.async.wait_group 0;" ::: "memory");      // (after an abort as well: nothing is in flight when the CTA leaves)
         while (told < issued) tell();
@@ -1072,9 +1092,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPpThreads, 1) atten
             // nothing more from here, and once it had completed the parity meant PV(j).)
             if (j >= 2 && !wait_all(bar(kPpPv + (j & 1)), (uint32_t)(((j - 2) >> 1) & 1))) { *abort_flag = 1u; break; }
             tc_fence_after();
-            const uint32_t t_sj = t_s + 64u * (uint32_t)(j & 1);
-            const int kbase = (kb_lo + j) << 6;
-            const bool all_seen = kbase >= rmin && kbase + 63 <= rmax;
+            const uint32_t t_sj = t_s + (uint32_t)S::kKeys * (uint32_t)(j & 1);
+            const int kbase = (kb_lo + j) << KB;
+            const bool all_seen = kbase >= rmin && kbase + S::kKeys - 1 <= rmax;
             // Scores of keys [32 c, + 32) of the block, masked.  TQ4: `factor`, the exponent's power of two, is still to be applied.  8-bit:
             // p.score_scale is, a constant operand (in one register with the power of two it made these builds spill, and a stack
             // frame costs this kernel several us a launch).
@@ -1112,12 +1132,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPpThreads, 1) atten
             };
             // TQ4 reads them twice (maximum, then weights): holding all 64 spills there (92 bytes a thread, five ragged
             // prompts 270 us instead of 245), while the 8-bit builds have room and the second read costs them 10 %.
-            constexpr int PARTS = DIRECT ? 1 : 2;      // 32-key parts of the block that this thread has
-            float sv[2][32];
+            float sv[2][32];      // two 32-key parts: the block's, or this thread's half of it
             float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};     // four independent chains
 #pragma unroll
-            for (int c = 0; c < PARTS; ++c) {
-                scores(c + half, sv[ROT ? 0 : c]);
+            for (int c = 0; c < 2; ++c) {
+                scores(c + 2 * half, sv[ROT ? 0 : c]);
 #pragma unroll
                 for (int i = 0; i < 32; ++i) mx4[i & 3] = fmaxf(mx4[i & 3], sv[ROT ? 0 : c][i]);
             }
@@ -1155,7 +1174,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPpThreads, 1) atten
             float ls4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
             const float m_use = ((m_ref < -1e29f) ? 0.0f : m_ref) - kPpShift;     // nothing visible yet: every P is 0
 #pragma unroll
-            for (int c = 0; c < PARTS; ++c) {
+            for (int c = 0; c < 2; ++c) {
                 uint32_t hi[16], lo[16];
                 if (ROT) scores(c, sv[0], true);
 #pragma unroll
@@ -1170,8 +1189,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPpThreads, 1) atten
                     lo[i] = pp_pack<FMT>(pa - hf.x, pb - hf.y);
                 }
                 // P takes the place of the scores it came from: value in columns 32 c .. + 15, residual in the next 16
-                tc_st16(t_sj + 32u * (c + half), hi);
-                tc_st16(t_sj + 32u * (c + half) + 16u, lo);
+                tc_st16(t_sj + 32u * (c + 2 * half), hi);
+                tc_st16(t_sj + 32u * (c + 2 * half) + 16u, lo);
             }
             tc_wait_st();
             l_run = l_run * alpha + ((ls4[0] + ls4[1]) + (ls4[2] + ls4[3]));
@@ -1235,13 +1254,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPpThreads, 1) atten
                 if (!fits) {
                     if constexpr (SCORED) {      // (the mass and rows of the other splits carry 2^kPpShift)
                         const ScoredRow one = {&p.layout, &p.batch, &p.sc, p.q_in, p.io_bf16, p.num_q_heads, p.gqa};
-                        scored_row_keys(one, place[0], q_off, q_head, place[1] << 6, ((place[1] + nblocks) << 6) - 1, 0, 1, v, m, l);
+                        scored_row_keys(one, place[0], q_off, q_head, place[1] << KB, ((place[1] + nblocks) << KB) - 1, 0, 1, v, m, l);
                         const float up = (float)(1 << (int)kPpShift);
                         l *= up;
 #pragma unroll
                         for (int i = 0; i < 8; ++i) v[i] *= ROT ? up * kPpLutScale : up;
                     } else if constexpr (!DIRECT) {
-                        prefill_row_fp32<FMT>(p, place[0], q_off, q_head, place[1] << 6, ((place[1] + nblocks) << 6) - 1, v, l, m);
+                        prefill_row_fp32<FMT>(p, place[0], q_off, q_head, place[1] << KB, ((place[1] + nblocks) << KB) - 1, v, l, m);
                     }
                 } else if (SCORED ? l != 0.0f : PpFormat<FMT>::has_keys(l)) {
                     const uint32_t qa = ROT ? quad_place(2u * lane) : 2u * lane;      // (the next quad is its neighbour)
