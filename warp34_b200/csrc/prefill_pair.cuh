@@ -1112,9 +1112,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPpThreads, 1) atten
                 }
                 if (SCORED && !again) {
                     const float away = (float)(g.ctx_before + q_off - (kbase + 32 * c));
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) sv[i] *= ROT ? factor : p.score_scale;
-                    change_scores(p.sc, sv, slope, [&](int i) { return away - (float)i; });
+                    change_scores(p.sc, sv, ROT ? factor : p.score_scale, slope, away);
                 }
                 if (!all_seen && !(SCORED && again)) {
 #pragma unroll
@@ -1138,7 +1136,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPpThreads, 1) atten
             for (int c = 0; c < 2; ++c) {
                 scores(c + 2 * half, sv[ROT ? 0 : c]);
 #pragma unroll
-                for (int i = 0; i < 32; ++i) mx4[i & 3] = fmaxf(mx4[i & 3], sv[ROT ? 0 : c][i]);
+                for (int i = 0; i < 32; ++i) {
+                    if (!SCORED) mx4[i & 3] = fmaxf(mx4[i & 3], sv[ROT ? 0 : c][i]);
+                    else if (i < 16) mx4[i & 3] = max_of(mx4[i & 3], sv[ROT ? 0 : c][2 * i], sv[ROT ? 0 : c][2 * i + 1]);
+                }
             }
             float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * (SCORED ? 1.0f : ROT ? factor : p.score_scale);
             if constexpr (DIRECT) {      // the row's other half: both threads go on with the same maximum
@@ -1172,6 +1173,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPpThreads, 1) atten
                 }
             }
             float ls4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            Two sums[2] = {0ull, 0ull};      // SCORED, in their place
             const float m_use = ((m_ref < -1e29f) ? 0.0f : m_ref) - kPpShift;     // nothing visible yet: every P is 0
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
@@ -1181,8 +1183,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPpThreads, 1) atten
                 for (int i = 0; i < 16; ++i) {
                     // masked scores are -infinity: ex2 gives exactly 0 against any finite reference
                     const float sa = sv[ROT ? 0 : c][2 * i], sb = sv[ROT ? 0 : c][2 * i + 1];
-                    const float pa = SCORED ? ex2(sa - m_use) : ex2(__fmaf_rn(sa, ROT ? factor : p.score_scale, -m_use));
-                    const float pb = SCORED ? ex2(sb - m_use) : ex2(__fmaf_rn(sb, ROT ? factor : p.score_scale, -m_use));
+                    if constexpr (SCORED) {      // two at a time
+                        const Two d = add_two(two_of(sa, sb), two_of(-m_use, -m_use)), w = two_of(ex2(first_of(d)), ex2(second_of(d)));
+                        sums[i & 1] = add_two(sums[i & 1], w);
+                        hi[i] = pp_pack<FMT>(first_of(w), second_of(w));
+                        const float2 hf = pp_unpack<FMT>(hi[i]);
+                        const Two rest = fma_two(two_of(hf.x, hf.y), two_of(-1.0f, -1.0f), w);
+                        lo[i] = pp_pack<FMT>(first_of(rest), second_of(rest));
+                        continue;
+                    }
+                    const float pa = ex2(__fmaf_rn(sa, ROT ? factor : p.score_scale, -m_use));
+                    const float pb = ex2(__fmaf_rn(sb, ROT ? factor : p.score_scale, -m_use));
                     ls4[i & 3] += pa + pb;
                     hi[i] = pp_pack<FMT>(pa, pb);
                     const float2 hf = pp_unpack<FMT>(hi[i]);
@@ -1193,6 +1204,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPpThreads, 1) atten
                 tc_st16(t_sj + 32u * (c + 2 * half) + 16u, lo);
             }
             tc_wait_st();
+            if (SCORED) {
+                const Two sum = add_two(sums[0], sums[1]);
+                ls4[0] = first_of(sum);
+                ls4[1] = second_of(sum);
+            }
             l_run = l_run * alpha + ((ls4[0] + ls4[1]) + (ls4[2] + ls4[3]));
             tc_fence_before();
             __syncwarp();
