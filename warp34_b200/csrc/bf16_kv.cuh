@@ -544,6 +544,8 @@ static int scored_configure() {
                                                 (int)PpSmem<WARP34_KV_FORMAT_Q8_0>::kBytes);
     if (rc == 0) rc = (int)cudaFuncSetAttribute(attention_prefill_pair_kernel<WARP34_KV_FORMAT_BF16, true>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                                 (int)PpSmem<WARP34_KV_FORMAT_BF16>::kBytes);
+    if (rc == 0) rc = (int)cudaFuncSetAttribute(scored_small_kernel<2>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)small_smem_bytes<2>());
+    if (rc == 0) rc = (int)cudaFuncSetAttribute(scored_small_kernel<3>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)small_smem_bytes<3>());
     if (rc == 0) done[dev] = true;
     return rc;
 }
@@ -574,6 +576,9 @@ static int launch_scored_attention(const warp34_exec* ex, const warp34_kv_layer_
     sc.slopes = change->distance_slopes;
     sc.key_begin = change->key_begin;
     sc.key_end = change->key_end;
+    if ((ex->flags & WARP34_B200_EXEC_FLAG_PRECISE_ATTENTION) == 0 && takes_small(layout, batch, num_q_heads)) {
+        return launch_scored_small(ex, layout, batch, sc, q_in, attn_out, num_q_heads, io_bf16);
+    }
     if (bf16) return launch_bf16_attention(ex, layout, batch, q_in, attn_out, num_q_heads, &sc);
     return launch_attention(ex, layout, batch, q_in, attn_out, nullptr, num_q_heads, io_bf16, -1, nullptr, &sc);
 }

@@ -1395,6 +1395,7 @@ W34_BOUNDS_HOST_HOOKS(attention)
 #include "tq4_stream_exact.cuh"
 #include "tq4_prefill_tc.cuh"
 #include "prefill_pair.cuh"
+#include "scored_small.cuh"
 #include "tq4_stream_tc.cuh"
 namespace w34 {
 
