@@ -163,17 +163,23 @@ __global__ void __launch_bounds__(kBfWarps * 32, 1) bf16kv_attention_stream_kern
         uint32_t qa[16][4];
         {
             __nv_bfloat16* stage = reinterpret_cast<__nv_bfloat16*>(ring_gen);   // [16][264]
-            for (int rr = 0; rr < kBfRows; ++rr) {
-                const int row = group * kBfRows + rr;
-                const int q_off = row / p.gqa;
-                const int q_head = kv_head * p.gqa + row % p.gqa;
-                const bool ok = row < rows_in_req &&
-                                (p.batch.valid_token_mask == nullptr || p.batch.valid_token_mask[g.q_start + q_off] != 0);
-                const size_t q_base = ((size_t)(g.q_start + q_off) * p.num_q_heads + q_head) * kHeadDim;
+            // 16 bytes a lane and row, eight rows on their way at once (row by row, two bytes a lane: 16 round trips to memory)
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const float x = ok ? load_act(p.q_in, q_base + lane + 32 * j, p.io_bf16) : 0.0f;
-                    stage[rr * 264 + lane + 32 * j] = __float2bfloat16_rn(x);
+            for (int r8 = 0; r8 < kBfRows; r8 += 8) {
+                uint32_t w[8][4];
+#pragma unroll
+                for (int rr = 0; rr < 8; ++rr) {
+                    const int row = group * kBfRows + r8 + rr;
+                    const int q_off = row / p.gqa;
+                    const int q_head = kv_head * p.gqa + row % p.gqa;
+                    const bool ok = row < rows_in_req &&
+                                    (p.batch.valid_token_mask == nullptr || p.batch.valid_token_mask[g.q_start + q_off] != 0);
+                    w[rr][0] = w[rr][1] = w[rr][2] = w[rr][3] = 0u;
+                    if (ok) load8_raw(p.q_in, ((size_t)(g.q_start + q_off) * p.num_q_heads + q_head) * kHeadDim, lane, w[rr]);
+                }
+#pragma unroll
+                for (int rr = 0; rr < 8; ++rr) {
+                    *reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(stage) + (r8 + rr) * kBfRowStride + 16 * lane) = make_uint4(w[rr][0], w[rr][1], w[rr][2], w[rr][3]);
                 }
             }
             __syncwarp();

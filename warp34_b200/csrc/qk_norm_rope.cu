@@ -13,7 +13,8 @@
 // position (a product in fp32 is off by 2^-7 rad at position 131072).  Sine and cosine are made once per token and block
 // (sincospif) and shared by its heads through shared memory, while the rows are on their way.
 //
-// Bound by HBM: 32768 tokens of 24 query heads with gate and 4 key heads (1745 MB) take 312 us, 0.87 of the measured copy rate.
+// Bound by HBM: 32768 tokens of 24 query heads with gate and 4 key heads (1745 MB) take 268 us, the measured copy rate; without a gate
+// (940 MB) 222 us, 0.66 of it, half of the issue slots taken.
 #include "tq4_common.cuh"
 
 #include <cuda_bf16.h>
@@ -21,6 +22,7 @@
 namespace w34 {
 
 constexpr int kQkWarps = 8;
+constexpr int kQkBlocks = 4;      // of eight warps an SM: registers of 32 rows of loads in flight
 
 struct QkParams {
     warp34_qk_norm_rope_args a;
@@ -66,8 +68,8 @@ __device__ __forceinline__ unsigned long long turns_of(float inv_freq) {
 }
 
 // Block: one token, (warps of the block) * ROWS of its head rows (blockIdx.y counts them).
-template <bool BF16, int ROWS>
-__global__ void __launch_bounds__(kQkWarps * 32) qk_norm_rope_kernel(const QkParams p) {
+template <bool BF16, int ROWS, bool GATED>
+__global__ void __launch_bounds__(kQkWarps * 32, kQkBlocks) qk_norm_rope_kernel(const QkParams p) {
     __shared__ __align__(16) float s_cos[kHeadDim / 2], s_sin[kHeadDim / 2];
     grid_dependency_wait();
     grid_launch_dependents();
@@ -76,17 +78,16 @@ __global__ void __launch_bounds__(kQkWarps * 32) qk_norm_rope_kernel(const QkPar
     const size_t tok = blockIdx.x;
     if (a.valid_token_mask != nullptr && a.valid_token_mask[tok] == 0) return;      // block-uniform
     const int warps = (int)(blockDim.x >> 5), row0 = (int)blockIdx.y * (warps * ROWS) + wid;
-    const bool gated = a.gate_out != nullptr;
-    const int q_width = gated ? 2 * kHeadDim : kHeadDim;
+    constexpr int q_width = GATED ? 2 * kHeadDim : kHeadDim;
 
-    uint32_t x[ROWS][4], gate[ROWS][4];
+    uint32_t x[ROWS][4], gate[GATED ? ROWS : 1][4];
 #pragma unroll
     for (int i = 0; i < ROWS; ++i) {
         const int row = row0 + warps * i;
         if (row < a.num_q_heads) {
             const uint16_t* src = static_cast<const uint16_t*>(a.q_in) + tok * (size_t)a.q_in_stride + (size_t)row * q_width + 8 * lane;
             qk_load8(src, p.aligned, x[i]);
-            if (gated) qk_load8(src + kHeadDim, p.aligned, gate[i]);
+            if (GATED) qk_load8(src + kHeadDim, p.aligned, gate[GATED ? i : 0]);
         } else if (row < p.rows) {
             qk_load8(static_cast<const uint16_t*>(a.k_in) + tok * (size_t)a.k_in_stride + (size_t)(row - a.num_q_heads) * kHeadDim + 8 * lane, p.aligned, x[i]);
         }
@@ -160,7 +161,7 @@ __global__ void __launch_bounds__(kQkWarps * 32) qk_norm_rope_kernel(const QkPar
         for (int k = 0; k < 4; ++k) out[k] = qk_narrow<BF16>(v[2 * k], v[2 * k + 1]);
         if (is_q) {
             qk_store8(static_cast<uint16_t*>(a.q_out) + tok * (size_t)a.q_out_stride + (size_t)row * kHeadDim + 8 * lane, p.aligned, out);
-            if (gated) qk_store8(static_cast<uint16_t*>(a.gate_out) + tok * (size_t)a.gate_out_stride + (size_t)row * kHeadDim + 8 * lane, p.aligned, gate[i]);
+            if (GATED) qk_store8(static_cast<uint16_t*>(a.gate_out) + tok * (size_t)a.gate_out_stride + (size_t)row * kHeadDim + 8 * lane, p.aligned, gate[GATED ? i : 0]);
         } else {
             qk_store8(static_cast<uint16_t*>(a.k_out) + tok * (size_t)a.k_out_stride + (size_t)(row - a.num_q_heads) * kHeadDim + 8 * lane, p.aligned, out);
         }
@@ -214,8 +215,12 @@ static int launch_qk_norm_rope(const warp34_exec* ex, const warp34_qk_norm_rope_
     const unsigned each = wide ? 4u : 1u, need = ((unsigned)rows + each - 1) / each, blocks = (need + kQkWarps - 1) / kQkWarps;
     const unsigned warps = (need + blocks - 1) / blocks;
     const dim3 grid((unsigned)a.num_tokens, blocks);
-    return wide ? launch_behind(qk_norm_rope_kernel<BF16, 4>, grid, warps * 32, 0, st, p)
-                : launch_behind(qk_norm_rope_kernel<BF16, 1>, grid, warps * 32, 0, st, p);
+    if (gated) {
+        return wide ? launch_behind(qk_norm_rope_kernel<BF16, 4, true>, grid, warps * 32, 0, st, p)
+                    : launch_behind(qk_norm_rope_kernel<BF16, 1, true>, grid, warps * 32, 0, st, p);
+    }
+    return wide ? launch_behind(qk_norm_rope_kernel<BF16, 4, false>, grid, warps * 32, 0, st, p)
+                : launch_behind(qk_norm_rope_kernel<BF16, 1, false>, grid, warps * 32, 0, st, p);
 }
 
 }  // namespace w34

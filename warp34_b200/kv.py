@@ -502,16 +502,16 @@ def paged_attention_scored(ex, layer, batch, q, out, num_q_heads, softcap=0.0, s
 
 def _head_rows(t, dtype, n, heads, width, what):
     """Checks that t is [n tokens, heads, width] with heads next to each other; returns its token stride."""
-    shape, stride = t.shape, t.stride()
-    if t.dtype is not dtype or len(shape) != 3 or shape[0] != n or shape[2] != width or (heads is not None and shape[1] != heads):
-        raise ValueError(f"{what}: expected {dtype} of shape [{n} tokens, heads, {width}], got {t.dtype} {tuple(shape)}")
-    if (stride[2] != 1 or (stride[1] != width and shape[1] > 1)) and t.numel() > 0:
+    if t.dtype is not dtype or t.shape != (n, heads, width):
+        raise ValueError(f"{what}: expected {dtype} of shape {(n, heads, width)}, got {t.dtype} {tuple(t.shape)}")
+    token, head, column = t.stride()
+    if (column != 1 or (head != width and heads > 1)) and t.numel() > 0:
         raise ValueError(f"{what}: heads must be contiguous")
-    return stride[0] if n > 1 else max(stride[0], shape[1] * width)
+    return token if n > 1 else heads * width
 
 
 def _norm_weight(w, dtype, what):
-    if w.dtype is not dtype or w.numel() != 256 or not w.is_contiguous():
+    if w.dtype is not dtype or w.shape != (256,) or w.stride() != (1,):
         raise ValueError(f"{what}_weight: 256 contiguous values of {dtype}")
     return w.data_ptr()
 
@@ -531,12 +531,12 @@ def qk_norm_rope(ex, q, k, q_weight, k_weight, positions, inv_freq, q_out, k_out
     q_in = q_to = q_w = k_in = k_to = k_w = gate_to = mask = pos = freq = None
     hq = hkv = qs = qos = ks = kos = gs = plane = rotary = planes = s1 = s2 = 0
     if q is not None:
-        hq = q.shape[1]
-        qs, qos = _head_rows(q, dtype, n, None, 256 if gate_out is None else 512, "q"), _head_rows(q_out, dtype, n, hq, 256, "q_out")
+        hq = q.shape[1] if q.dim() == 3 else 0
+        qs, qos = _head_rows(q, dtype, n, hq, 256 if gate_out is None else 512, "q"), _head_rows(q_out, dtype, n, hq, 256, "q_out")
         q_in, q_to, q_w = q.data_ptr(), q_out.data_ptr(), _norm_weight(q_weight, dtype, "q")
     if k is not None:
-        hkv = k.shape[1]
-        ks, kos = _head_rows(k, dtype, n, None, 256, "k"), _head_rows(k_out, dtype, n, hkv, 256, "k_out")
+        hkv = k.shape[1] if k.dim() == 3 else 0
+        ks, kos = _head_rows(k, dtype, n, hkv, 256, "k"), _head_rows(k_out, dtype, n, hkv, 256, "k_out")
         k_in, k_to, k_w = k.data_ptr(), k_out.data_ptr(), _norm_weight(k_weight, dtype, "k")
     if gate_out is not None:
         _require(q is not None, "qk_norm_rope: a gate without queries")
