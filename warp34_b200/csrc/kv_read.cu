@@ -13,10 +13,12 @@
 // X comes as fp16 value and residual from a table by code byte (22 bits of a centroid), Z is split the same way: eight products a row.
 // The accumulators of the first are the A fragments of the second as they lie in the lanes; columns of the first +-1 matrix are ordered so
 // that a lane's elements are four neighbouring columns (two code bytes).  The rounded row passes through shared memory (stmatrix,
-// transposed), so that a lane stores 16 bytes.  (With movmatrix instead of that, 8 bytes a lane: 55 us.)
+// transposed), so that a lane stores 16 bytes.  (With movmatrix instead of that and 8 bytes a lane 124 instructions a row, 23 of them on the shared-memory pipe instead of 12.)
 // (Eight lanes to a row, the transform in packed fp32 arithmetic and its columns changing lanes through shared memory: 67 us instead of
-// 55 for 35065 tokens of 4 heads, at 40 shared-memory wavefronts and 168 instructions a row.)
-// Bound by instruction issue (118 a row, 60 % of the slots) and by the latency of the rows' loads (a third of the stalls); HBM is at 26 %.
+// 52 for 35065 tokens of 4 heads, at 40 shared-memory wavefronts and 168 instructions a row.)
+// Bound by instruction issue: 119 a row, two thirds of the slots with 24 warps an SM; HBM is at 0.54 of the copy rate.  8-bit and BF16 rows,
+// 0.7 and 0.8 of it.  The rows of a warp's next token are on their way while it computes (57 instead of 61 us with a cold L2; with the
+// registers of four blocks an SM instead of three they spill).
 #include "tq4_common.cuh"
 
 #include <cuda_bf16.h>
@@ -25,7 +27,7 @@
 namespace w34 {
 
 constexpr int kReadWarps = 8;
-constexpr int kReadTq4Blocks = 4;              // resident blocks an SM that a grid is sized for
+constexpr int kReadTq4Blocks = 3;              // resident blocks an SM that a grid is sized for
 constexpr int kReadRows = 4;                   // rows of a warp on their way at once: heads of one token
 constexpr int kReadTableBytes = 256 * 128;     // byte -> (value pair, residual pair), 16 copies
 
@@ -69,12 +71,28 @@ __device__ __forceinline__ uint32_t read_half2(float a, float b) {
     const __half2 v = __floats2half2_rn(a, b);
     return *reinterpret_cast<const uint32_t*>(&v);
 }
+// Two numbers in packed arithmetic, each rounded as the scalar instruction does.
+typedef unsigned long long Two;
+__device__ __forceinline__ Two two_of(float a, float b) { return (Two)__float_as_uint(a) | ((Two)__float_as_uint(b) << 32); }
+__device__ __forceinline__ float first_of(Two p) { return __uint_as_float((uint32_t)p); }
+__device__ __forceinline__ float second_of(Two p) { return __uint_as_float((uint32_t)(p >> 32)); }
+__device__ __forceinline__ Two mul_two(Two a, Two b) {
+    Two r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ Two fma_two(Two a, Two b, Two c) {
+    Two r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
 // a and b as fp16 pairs of values and of residuals.  The value is cut off, not rounded (one instruction, and exactly what the pair then holds):
 // the residual is below 2^-10 of it and keeps 11 bits of its own.
 __device__ __forceinline__ void read_split(float a, float b, uint32_t& value, uint32_t& residual) {
     const float va = __uint_as_float(__float_as_uint(a) & 0xffffe000u), vb = __uint_as_float(__float_as_uint(b) & 0xffffe000u);
     value = read_half2(va, vb);
-    residual = read_half2(a - va, b - vb);
+    const Two rest = fma_two(two_of(va, vb), two_of(-1.0f, -1.0f), two_of(a, b));
+    residual = read_half2(first_of(rest), second_of(rest));
 }
 // Entries (i, j0), (i, j1) of the 16-point Walsh-Hadamard matrix times `scale`, as an fp16 pair.
 __device__ __forceinline__ uint32_t read_hadamard(int i, int j0, int j1, float scale) {
@@ -179,32 +197,46 @@ __global__ void __launch_bounds__(kReadWarps * 32, kReadTq4Blocks) kv_read_tq4_k
     const ReadShare share(p);
     uint64_t rows = 0;
     uint16_t* dst = p.out[side] + (size_t)share.first * (size_t)p.stride[side] + (head0 * kHeadDim + 8 * lane);
-#pragma unroll 1
-    for (int t = share.first; t < share.end; ++t, dst += p.stride[side]) {
-        const int k32 = (t - share.first) & 31;
-        if (k32 == 0) rows = read_rows_of(p, t, share.end, head0, side);
-        const uint8_t* row = reinterpret_cast<const uint8_t*>((uintptr_t)__shfl_sync(0xffffffffu, rows, k32));
-        if (row == nullptr) continue;
-        uint32_t codes[ROWS][2], scales[ROWS][2];      // fp16 bits of the scales
+    // Codes and scales (fp16 bits) of a token's rows; those of the next token are on their way while a token's are computed.
+    struct Raw { uint32_t codes[ROWS][2], scales[ROWS][2]; };
+    auto load = [&](Raw& raw, uint64_t at) {
+        const uint8_t* row = reinterpret_cast<const uint8_t*>((uintptr_t)at);
 #pragma unroll
         for (int i = 0; i < ROWS; ++i) {
-            if (ROWS > 1 && i >= n_rows) break;
+            if (at == 0 || (ROWS > 1 && i >= n_rows)) break;
             const uint8_t* mine = row + (2 + 8 * gid + 2 * tig);
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                codes[i][h] = *reinterpret_cast<const uint16_t*>(mine + kTq4BlockBytes * h);
-                scales[i][h] = *reinterpret_cast<const uint16_t*>(row + kTq4BlockBytes * h);
+                raw.codes[i][h] = *reinterpret_cast<const uint16_t*>(mine + kTq4BlockBytes * h);
+                raw.scales[i][h] = *reinterpret_cast<const uint16_t*>(row + kTq4BlockBytes * h);
             }
             row += head_stride;
         }
+    };
+    uint64_t at_next = 0;
+    Raw next = {};
+    if (share.first < share.end) {
+        rows = read_rows_of(p, share.first, share.end, head0, side);
+        at_next = __shfl_sync(0xffffffffu, rows, 0);
+        load(next, at_next);
+    }
+#pragma unroll 1
+    for (int t = share.first; t < share.end; ++t, dst += p.stride[side]) {
+        const uint64_t at = at_next;
+        const Raw raw = next;
+        const int k32 = (t + 1 - share.first) & 31;
+        if (k32 == 0 && t + 1 < share.end) rows = read_rows_of(p, t + 1, share.end, head0, side);
+        at_next = t + 1 < share.end ? __shfl_sync(0xffffffffu, rows, k32) : 0;
+        load(next, at_next);
+        if (at == 0) continue;
 #pragma unroll
         for (int i = 0; i < ROWS; ++i) {
             if (ROWS > 1 && i >= n_rows) break;
             float u[2][4];
 #pragma unroll
             for (int h = 0; h < 2; ++h) {      // the half with scale d[h]: a = 8 h + n
-                const uint2 e0 = *reinterpret_cast<const uint2*>(table + (((codes[i][h] << 7) & 0x7f80u) | copy));
-                const uint2 e1 = *reinterpret_cast<const uint2*>(table + (((codes[i][h] >> 1) & 0x7f80u) | copy));
+                const uint2 e0 = *reinterpret_cast<const uint2*>(table + (((raw.codes[i][h] << 7) & 0x7f80u) | copy));
+                const uint2 e1 = *reinterpret_cast<const uint2*>(table + (((raw.codes[i][h] >> 1) & 0x7f80u) | copy));
                 float z[4];
                 read_mma_zero(z, ha[0], ha[1], ha[2], ha[3], e0.x, e1.x);
                 read_mma(z, ha[0], ha[1], ha[2], ha[3], e0.y, e1.y);
@@ -214,15 +246,14 @@ __global__ void __launch_bounds__(kReadWarps * 32, kReadTq4Blocks) kv_read_tq4_k
                 read_mma8_zero(u[h], v0, v1, hb);
                 read_mma8(u[h], r0, r1, hb);
             }
-            const float d0 = __half2float(__ushort_as_half((unsigned short)scales[i][0])), d1 = __half2float(__ushort_as_half((unsigned short)scales[i][1]));
-#pragma unroll
-            for (int k = 0; k < 4; ++k) u[0][k] *= d0;
+            const float d0 = __half2float(__ushort_as_half((unsigned short)raw.scales[i][0])), d1 = __half2float(__ushort_as_half((unsigned short)raw.scales[i][1]));
             uint32_t w[2][2];      // matrices (a' 8 n .., b' 8 m ..)
 #pragma unroll
-            for (int n = 0; n < 2; ++n) {
-                const float d = n ? -d1 : d1;
-#pragma unroll
-                for (int m = 0; m < 2; ++m) w[n][m] = read_narrow<BF16>(__fmaf_rn(d, u[1][2 * m], u[0][2 * m]), __fmaf_rn(d, u[1][2 * m + 1], u[0][2 * m + 1]));
+            for (int m = 0; m < 2; ++m) {
+                const Two low = mul_two(two_of(u[0][2 * m], u[0][2 * m + 1]), two_of(d0, d0)), high = two_of(u[1][2 * m], u[1][2 * m + 1]);
+                const Two sum = fma_two(high, two_of(d1, d1), low), difference = fma_two(high, two_of(-d1, -d1), low);
+                w[0][m] = read_narrow<BF16>(first_of(sum), second_of(sum));
+                w[1][m] = read_narrow<BF16>(first_of(difference), second_of(difference));
             }
             __syncwarp();      // the row before has been read
             asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};"
