@@ -304,7 +304,8 @@ def _prepare_project(case, seed):
          "weights": weights, "pos": pos, "inv_freq": inv_freq}
     if own:
         from warp34_b200 import kv
-        s.update(ex=kv.Executor(1 << 16), q_out=new(hq), k_out=new(hkv), gate_out=new(hq) if case["gate"] else None)
+        s.update(ex=kv.Executor(1 << 16), q_out=new(hq), k_out=new(hkv), gate_out=new(hq) if case["gate"] else None,
+                 sections=_axes(case["rotary"], 3)[1] if case["planes"] == 3 else None)
     return s
 
 
@@ -339,9 +340,8 @@ def _own_attend(s):
 
 def _own_project(s):
     from warp34_b200 import kv
-    sections = _axes(s["case"]["rotary"], 3)[1] if s["case"]["planes"] == 3 else None
     kv.qk_norm_rope(s["ex"], s["q"], s["k"], s["weights"][0], s["weights"][1], s["pos"], s["inv_freq"], s["q_out"], s["k_out"],
-                    gate_out=s["gate_out"], sections=sections, eps=EPS, weight_offset=1.0)
+                    gate_out=s["gate_out"], sections=s["sections"], eps=EPS, weight_offset=1.0)
     return [s["q_out"], s["k_out"], s["gate_out"]] if s["case"]["gate"] else [s["q_out"], s["k_out"]]
 
 
