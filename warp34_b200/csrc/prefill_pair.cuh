@@ -1268,16 +1268,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPpThreads, 1) atten
                 float l = DIRECT ? src[256] + src[258] : src[256], m = src[257];
                 float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
                 if (!fits) {
-                    if constexpr (SCORED) {      // (the mass and rows of the other splits carry 2^kPpShift)
+                    if constexpr (SCORED) {
                         const ScoredRow one = {&p.layout, &p.batch, &p.sc, p.q_in, p.io_bf16, p.num_q_heads, p.gqa};
                         scored_row_keys(one, place[0], q_off, q_head, place[1] << KB, ((place[1] + nblocks) << KB) - 1, 0, 1, v, m, l);
-                        const float up = (float)(1 << (int)kPpShift);
-                        l *= up;
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) v[i] *= ROT ? up * kPpLutScale : up;
+                        for (int i = 0; i < 8; ++i) v[i] *= ROT ? kPpLutScale : 1.0f;
                     } else if constexpr (!DIRECT) {
                         prefill_row_fp32<FMT>(p, place[0], q_off, q_head, place[1] << KB, ((place[1] + nblocks) << KB) - 1, v, l, m);
                     }
+                    // the mass and rows of the other key ranges carry 2^kPpShift
+                    const float up = (float)(1 << (int)kPpShift);
+                    l *= up;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) v[i] *= up;
                 } else if (SCORED ? l != 0.0f : PpFormat<FMT>::has_keys(l)) {
                     const uint32_t qa = ROT ? quad_place(2u * lane) : 2u * lane;      // (the next quad is its neighbour)
                     const float4 a = *reinterpret_cast<const float4*>(src + 4u * qa), b = *reinterpret_cast<const float4*>(src + 4u * (qa ^ 1u));
