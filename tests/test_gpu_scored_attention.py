@@ -77,6 +77,8 @@ SHAPES = {
     "stream_gqa1": (3, 3, [1] * 9, [4, 100, 31, 32, 33, 0, 511, 62, 63]),
     "stream_verify": (6, 1, [3, 2, 4, 4, 4, 3], [40, 500, 0, 60, 100, 7]),
     "stream_long": (6, 1, [1], [2500]),
+    "stream_long_batch": (16, 4, [1] * 9, [2047, 5, 64, 1000, 33, 700, 129, 300, 16]),
+    "stream_long_verify": (4, 1, [4, 2, 4], [21900, 40, 900]),
     # a few tokens over short contexts: one launch
     "small_eight_rows": (8, 1, [1, 2], [1020, 100]),
     "small_five_rows": (5, 1, [2, 1], [100, 255]),
@@ -135,7 +137,7 @@ def test_symmetric_window_and_negative_scale(env, name):
 
 
 @pytest.mark.parametrize("name", FORMATS)
-@pytest.mark.parametrize("shape", ["four_rows", "verify", "chunks", "stream_four_rows", "stream_verify"])
+@pytest.mark.parametrize("shape", ["four_rows", "verify", "chunks", "stream_four_rows", "stream_verify", "stream_long_batch"])
 def test_masked_rows_are_left_alone(env, name, shape):
     hq, hkv, lens, ctx = SHAPES[shape]
     cache = Cache(name, hkv, lens, ctx, seed=8, tail=0xff)
@@ -220,19 +222,20 @@ def _spoil(cache, r, pos, side, value):
 
 @pytest.mark.parametrize("value", [np.nan, np.inf])
 @pytest.mark.parametrize("side", [0, 1])
-@pytest.mark.parametrize("shape", ["decode", "verify", "chunk", "chunk_cut", "stream_verify"])
+@pytest.mark.parametrize("shape", ["decode", "verify", "chunk", "chunk_cut", "stream_verify", "stream_long_verify"])
 @pytest.mark.parametrize("name", FORMATS)
 def test_non_finite_rows_reach_only_the_rows_that_see_them(env, name, shape, side, value):
     """A NaN or infinity in K or V of one document: tokens of the others, in the same tile, have the results they would have without it."""
     hq, hkv, lens, ctx = {"decode": (4, 2, [1, 1], [60, 61]), "verify": (4, 1, [4, 2], [58, 60]), "chunk": (4, 2, [90, 64], [33, 0]),
-                          "chunk_cut": (2, 1, [40], [2000]), "stream_verify": (4, 1, [4, 2, 4, 4, 4, 4, 4], [58, 60, 57, 58, 59, 58, 57])}[shape]
+                          "chunk_cut": (2, 1, [40], [2000]), "stream_verify": (4, 1, [4, 2, 4, 4, 4, 4, 4], [58, 60, 57, 58, 59, 58, 57]),
+                          "stream_long_verify": (4, 1, [4, 4, 4], [21998, 19998, 30])}[shape]
     cache = Cache(name, hkv, lens, ctx, seed=31, tail=0xff)
     q = _queries(name, sum(lens), hq, 16)
     pos = np.concatenate([c + np.arange(m) for c, m in zip(ctx, lens)])
-    doc = {"decode": 61, "verify": 60, "chunk": 50, "chunk_cut": 2010, "stream_verify": 60}[shape]
+    doc = {"decode": 61, "verify": 60, "chunk": 50, "chunk_cut": 2010, "stream_verify": 60, "stream_long_verify": 2000}[shape]
     key_begin, key_end = (pos // doc * doc).astype(np.int32), (pos + 1).astype(np.int32)
     clean, size = scored_attention(cache, q.float().numpy(), hq, softcap=30.0, key_begin=key_begin, key_end=key_end)
-    spoiled = {"decode": 10, "verify": 59, "chunk": 49, "chunk_cut": 2004, "stream_verify": 59}[shape]
+    spoiled = {"decode": 10, "verify": 59, "chunk": 49, "chunk_cut": 2004, "stream_verify": 59, "stream_long_verify": 21999}[shape]
     for r in range(len(lens)):
         _spoil(cache, r, min(spoiled, ctx[r] + lens[r] - 1), side, value)
     cache.upload()

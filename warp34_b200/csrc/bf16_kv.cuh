@@ -420,23 +420,28 @@ extern "C" size_t warp34_paged_attention_bf16_scratch_bytes(const warp34_kv_laye
 }
 
 namespace w34 {
-// Scored attention over BF16 layers: which kernel serves a call.  The CTA-pair kernel takes chunks (more than 16 query rows per kv head in some
-// request: the stream kernel reads a request's pages once for every 16, the pair kernel once for 256), the stream kernel the rest where
-// the workspace holds the plan, the items and one CTA's partials, the row kernel what neither takes.
+// Scored attention over BF16 layers: which kernel serves a call.  The CTA-pair kernel reads a request's pages once for 256 rows, in one launch, but
+// takes as long for one row; the stream kernel once for every 16 and spreads them over the whole GPU, in three.  By rows of the longest request
+// and (request, kv head, key) units.  Measured, stream / pair, us with a cold L2, requests of n keys on 4 kv heads: up to 16 rows, 1 x 8000 53 / 37,
+// 8 x 1000 37 / 35, 1 x 30000 59 / 74, 32 x 1000 57 / 86, 8 x 8000 88 / 135 (on one kv head 8 x 8000 57 / 49); 17 to 32 rows, 32 x 1000 84 / 90,
+// 1 x 30000 86 / 78, 8 x 8000 127 / 139, 32 x 8000 387 / 483; 48 rows, 8 x 8000 154 / 137, 32 x 8000 527 / 467.  Without a
+// workspace for the plan, the items and one CTA's partials the pair kernel serves all; the row kernel what neither does (other alignments, more than
+// 128 query heads to a kv head, WARP34_B200_EXEC_FLAG_PRECISE_ATTENTION).
 enum Bf16Route { kBf16Rows, kBf16Stream, kBf16Pair };
-static Bf16Route bf16_scored_route(const warp34_exec* ex, const warp34_kv_layer_layout* layout, const warp34_attention_batch* batch, int num_q_heads, int* rc) {
+static Bf16Route bf16_scored_route(const warp34_exec* ex, const warp34_kv_layer_layout* layout, const warp34_attention_batch* batch, int num_q_heads) {
     if ((ex->flags & WARP34_B200_EXEC_FLAG_PRECISE_ATTENTION) != 0 || !bf16_strides_aligned16(layout)) return kBf16Rows;
     const int gqa = num_q_heads / layout->local_kv_heads;
-    if (gqa <= kPpCtaRows && (long long)batch->max_q_len * gqa > kBfRows) {
-        *rc = bf16kv_configure();
-        return kBf16Pair;
-    }
+    const long long rows = (long long)(batch->max_q_len > 0 ? batch->max_q_len : 1) * gqa;
+    long long keys = batch->max_seq_len > 0 ? (long long)batch->max_seq_len : (long long)batch->max_blocks_per_req * kPageTokens;
+    if (batch->sliding_window > 0 && (long long)batch->sliding_window + batch->max_q_len < keys) keys = (long long)batch->sliding_window + batch->max_q_len;
+    const long long units = (long long)batch->num_reqs * layout->local_kv_heads * keys;
+    if (gqa <= kPpCtaRows && units <= (rows <= kBfRows ? 65536ll : rows <= 2 * kBfRows ? 200000ll : 0x7fffffffffffffffll)) return kBf16Pair;
     const long long items = items_bound(layout, batch, num_q_heads, kBfRows);
     const size_t plan = plan_bytes(batch->num_reqs);
     const size_t avail = ex->scratch_size > plan ? ex->scratch_size - plan : 0;
     const long long workers = (long long)(avail / ((size_t)(kBfRows * kHeadDim + 2 * kBfRows) * sizeof(float))) - items;
-    if (ex->scratch_ptr == 0 || (ex->scratch_ptr & 15u) != 0 || workers < kBfWarps || items * (long long)batch->max_blocks_per_req >= 0x7fffffffll) return kBf16Rows;
-    return kBf16Stream;
+    const bool stream = ex->scratch_ptr != 0 && (ex->scratch_ptr & 15u) == 0 && workers >= kBfWarps && items * (long long)batch->max_blocks_per_req < 0x7fffffffll;
+    return stream ? kBf16Stream : gqa <= kPpCtaRows ? kBf16Pair : kBf16Rows;
 }
 }  // namespace w34
 
@@ -457,8 +462,7 @@ static int launch_bf16_attention(const warp34_exec* ex, const warp34_kv_layer_la
     if (layout->head_dim != kHeadDim || layout->block_size != kPageTokens) return (int)cudaErrorNotSupported;
     if (sc != nullptr) {
         int rc = 0;
-        const Bf16Route route = bf16_scored_route(ex, layout, batch, num_q_heads, &rc);
-        if (rc != 0) return rc;
+        const Bf16Route route = bf16_scored_route(ex, layout, batch, num_q_heads);
         if (route == kBf16Rows) return launch_scored_rows(ex, layout, batch, *sc, q_in, attn_out, num_q_heads, 1);
         if (route == kBf16Pair) {
             const OutputGate none = {nullptr, 0};
