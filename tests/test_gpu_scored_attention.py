@@ -76,7 +76,8 @@ SHAPES = {
     "stream_six_rows": (24, 4, [1] * 6, [255, 1, 90, 1000, 47, 48]),
     "stream_gqa1": (3, 3, [1] * 9, [4, 100, 31, 32, 33, 0, 511, 62, 63]),
     "stream_verify": (6, 1, [3, 2, 4, 4, 4, 3], [40, 500, 0, 60, 100, 7]),
-    "stream_long": (6, 1, [1], [2500]),
+    "stream_long": (6, 1, [1], [33000]),
+    "stream_six_rows_long": (24, 4, [1] * 5, [2047, 255, 90, 1000, 47]),
     "stream_long_batch": (16, 4, [1] * 9, [2047, 5, 64, 1000, 33, 700, 129, 300, 16]),
     "stream_long_verify": (4, 1, [4, 2, 4], [21900, 40, 900]),
     # a few tokens over short contexts: one launch
@@ -191,7 +192,7 @@ def test_the_row_kernel(env, name, how):
 
 
 @pytest.mark.parametrize("name", ["tq4"])
-@pytest.mark.parametrize("shape", ["one", "verify", "chunks", "stream_six_rows", "stream_verify"])
+@pytest.mark.parametrize("shape", ["one", "verify", "chunks", "stream_six_rows", "stream_six_rows_long", "stream_long_verify"])
 def test_bf16_activations_over_tq4(env, name, shape):
     hq, hkv, lens, ctx = SHAPES[shape]
     cache = Cache(name, hkv, lens, ctx, seed=8, tail=0xff)
@@ -260,7 +261,7 @@ def test_non_finite_rows_reach_only_the_rows_that_see_them(env, name, shape, sid
 def test_less_workspace_gives_the_same_results(env, name):
     """A workspace for part of the requests at a time, and one that holds nothing but the row kernel's needs."""
     kv = env["kv"]
-    hq, hkv, lens, ctx = 24, 4, [1] * 40, [5 * i for i in range(40)]
+    hq, hkv, lens, ctx = 24, 4, [1] * 40, [7 * i for i in range(40)]
     cache = Cache(name, hkv, lens, ctx, seed=41, tail=0xff)
     q = _queries(name, 40, hq, 17)
     kw, window = _change("all", hq, lens, ctx, 6)
@@ -276,7 +277,7 @@ def test_less_workspace_gives_the_same_results(env, name):
 
 
 @pytest.mark.parametrize("name", FORMATS)
-@pytest.mark.parametrize("shape", ["four_rows", "chunks", "stream_six_rows"])
+@pytest.mark.parametrize("shape", ["four_rows", "chunks", "stream_six_rows", "stream_long_batch"])
 def test_capture_replay_streams_and_repeatability(env, name, shape):
     kv = env["kv"]
     hq, hkv, lens, ctx = SHAPES[shape]

@@ -432,9 +432,7 @@ static Bf16Route bf16_scored_route(const warp34_exec* ex, const warp34_kv_layer_
     if ((ex->flags & WARP34_B200_EXEC_FLAG_PRECISE_ATTENTION) != 0 || !bf16_strides_aligned16(layout)) return kBf16Rows;
     const int gqa = num_q_heads / layout->local_kv_heads;
     const long long rows = (long long)(batch->max_q_len > 0 ? batch->max_q_len : 1) * gqa;
-    long long keys = batch->max_seq_len > 0 ? (long long)batch->max_seq_len : (long long)batch->max_blocks_per_req * kPageTokens;
-    if (batch->sliding_window > 0 && (long long)batch->sliding_window + batch->max_q_len < keys) keys = (long long)batch->sliding_window + batch->max_q_len;
-    const long long units = (long long)batch->num_reqs * layout->local_kv_heads * keys;
+    const long long units = scored_units(layout, batch);
     if (gqa <= kPpCtaRows && units <= (rows <= kBfRows ? 65536ll : rows <= 2 * kBfRows ? 200000ll : 0x7fffffffffffffffll)) return kBf16Pair;
     const long long items = items_bound(layout, batch, num_q_heads, kBfRows);
     const size_t plan = plan_bytes(batch->num_reqs);

@@ -2059,6 +2059,18 @@ static Kv8Route kv8_chunk_route(const warp34_exec* ex, const warp34_kv_layer_lay
     return both < pair_all ? kKv8Both : kKv8Pair;
 }
 
+// Scored attention: the (request, kv head, key) units of a call at most, by what the host knows.
+static long long scored_units(const warp34_kv_layer_layout* l, const warp34_attention_batch* b) {
+    long long keys = b->max_seq_len > 0 ? (long long)b->max_seq_len : (long long)b->max_blocks_per_req * kPageTokens;
+    if (b->sliding_window > 0 && (long long)b->sliding_window + b->max_q_len < keys) keys = (long long)b->sliding_window + b->max_q_len;
+    return (long long)b->num_reqs * l->local_kv_heads * keys;
+}
+// Up to so many, the CTA-pair kernel also takes requests of few rows: one launch instead of three.  Measured, stream / pair, us with a cold L2, TQ4
+// requests of n keys on 4 kv heads: 8 x 100 38 / 27, 1 x 8000 48 / 46, 8 x 1000 48 / 46, 32 x 100 44 / 45, 1 x 30000 58 / 93, 32 x 1000 58 / 117 (four drafted
+// tokens on 6 rows each: 42 / 27, 56 / 48, 58 / 50, 58 / 45, 87 / 101, 93 / 123).  FP8, whose stream kernel needs no query fragments: 8 x 100 24 / 21, 1 x 8000
+// 32 / 42, 8 x 1000 32 / 42.
+constexpr long long kScoredPairUnitsTq4 = 32768, kScoredPairUnitsKv8 = 4096;
+
 static bool takes_kv8_chunk_path(uint64_t flags, const warp34_kv_layer_layout* l, const warp34_attention_batch* b, int num_q_heads) {
     if ((flags & WARP34_B200_EXEC_FLAG_PRECISE_ATTENTION) != 0 || !kv8_canonical(l) || l->k_base == 0 || l->v_base == 0 ||
         l->local_kv_heads <= 0 || num_q_heads % l->local_kv_heads != 0 || b->num_reqs <= 0 || b->block_tables == nullptr ||
@@ -2091,6 +2103,15 @@ static int launch_attention(const warp34_exec* ex, const warp34_kv_layer_layout*
     if (batch->total_tokens <= 0 || num_q_heads <= 0) return 0;
     if (kv8_attention_layout_ok(layout)) {   // unrotated 8-bit boundary layers; a decode batch's epilogue is a second launch, in place
         if (triple_out != nullptr) return (int)cudaErrorNotSupported;
+        if (sc != nullptr && (ex->flags & WARP34_B200_EXEC_FLAG_PRECISE_ATTENTION) == 0 && kv8_canonical(layout) && num_q_heads / layout->local_kv_heads <= kPpCtaRows &&
+            scored_units(layout, batch) <= kScoredPairUnitsKv8) {
+            int rc = 0;
+            const DeviceInfo* dev = device_info(&rc);
+            if (dev == nullptr) return rc;
+            return layout->k_format == WARP34_KV_FORMAT_FP8_E4M3
+                       ? launch_prefill_pair<WARP34_KV_FORMAT_FP8_E4M3, true>(ex, layout, batch, q_in, attn_out, num_q_heads, io_bf16, og, dev->sm_count, 0, *sc)
+                       : launch_prefill_pair<WARP34_KV_FORMAT_Q8_0, true>(ex, layout, batch, q_in, attn_out, num_q_heads, io_bf16, og, dev->sm_count, 0, *sc);
+        }
         if (force <= 0 && takes_kv8_chunk_path(ex->flags, layout, batch, num_q_heads)) {
             int rc = 0;
             const DeviceInfo* dev = device_info(&rc);
@@ -2141,7 +2162,9 @@ static int launch_attention(const warp34_exec* ex, const warp34_kv_layer_layout*
     // flag (or the tcgen05-verify flag) tcgen05 + TMEM with single fp16 operands.
     const bool chunk_geometry_ok = stream_layout_ok(layout) && batch->max_blocks_per_req > 0 && gqa <= kPpCtaRows;
     if (force >= 1 && (!chunk_geometry_ok || triple_out != nullptr)) return (int)cudaErrorNotSupported;
-    if (force >= 1 || (force < 0 && triple_out == nullptr && takes_prefill_path(ex->flags, layout, batch, gqa))) {
+    const bool few_units = sc != nullptr && (ex->flags & WARP34_B200_EXEC_FLAG_PRECISE_ATTENTION) == 0 && chunk_geometry_ok &&
+                           scored_units(layout, batch) <= kScoredPairUnitsTq4;
+    if (force >= 1 || few_units || (force < 0 && triple_out == nullptr && takes_prefill_path(ex->flags, layout, batch, gqa))) {
         const bool tc = sc == nullptr && (force == 2 || (force < 0 && (ex->flags & (WARP34_B200_EXEC_FLAG_FAST_ATTENTION |
                                                                   WARP34_B200_EXEC_FLAG_TCGEN05_VERIFY)) != 0));
         if (sc != nullptr) {
