@@ -106,7 +106,13 @@ __device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((u
 
 // BF16 rows are operands as they are: no residual parts and no raw stages (the producers copy rows straight into the tiles).  That leaves
 // room for the query in shared memory, and its columns of tensor memory for blocks of 128 keys, over which the waits and exchanges of a block
-// are spread (64 keys with the query in tensor memory: 3.3 ms for 8 x 2048 tokens after 8192, 128 2.8).
+// are spread (64 keys with the query in tensor memory: 3.3 ms for 8 x 2048 tokens after 8192, 128 2.8, both uncapped).
+//   warps 0-7   consumers: two threads a row, each with one half of the keys of either half of a block; their maxima meet in shared memory
+//   warps 8-9   K, warps 10-11 V: rows copied to their swizzled places, 16 bytes a lane (cp.async)
+//   warp 12     as above; the output product of a block's first half starts as soon as that half's weights are there
+//               (both halves at once: 964 instead of 937 us for 4 x 2048 capped tokens after 2048, 24 / 4 heads)
+// What bounds it: capped, the consumers (three special functions a score against one) and the power cap: 8 x 2048 tokens after 8192
+// take 3.3 to 3.5 ms capped and 2.8 ms = 880 TFLOP/s uncapped.
 template <int FMT> struct PpSmem {
     static constexpr bool kDirect = FMT == WARP34_KV_FORMAT_BF16;
     static constexpr int kStages = kDirect ? 4 : kPpStages;
@@ -136,7 +142,7 @@ template <int FMT> struct PpSmem {
     // barrier slots (8 bytes each).  Full / PReady: waited for by the MMA warp of CTA 0, arrivals from both CTAs.
     // Empty, S, Pv: one arrival per CTA from the MMA warp's commits.  Raw*: within a CTA.
     enum { FullK = 0, FullV = FullK + kStages, EmptyK = FullV + kStages, EmptyV = EmptyK + kStages, SReady = EmptyV + kStages, PReady = SReady + 2,
-           Pv = PReady + 2, Drain = Pv + 2, RawKFull, RawKFree = RawKFull + kPpRawStages, RawVFull = RawKFree + kPpRawStages,
+           Pv = PReady + (kDirect ? 4 : 2), Drain = Pv + 2, RawKFull, RawKFree = RawKFull + kPpRawStages, RawVFull = RawKFree + kPpRawStages,
            RawVFree = RawVFull + kPpRawStages, Halves = RawVFree + kPpRawStages,
            BarCount = Halves + (kDirect ? 4 : 0) };
     static_assert((uint32_t)BarCount * 8u <= kWords, "barrier slots end before the words behind them");
@@ -519,7 +525,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPpThreads, 1) atten
         mbar_init(bar(kPpPv + 1), 1u);
         mbar_init(bar(kPpPReady), 2u * S::kConsumers);       // the consumer warps of both CTAs
         mbar_init(bar(kPpPReady + 1), 2u * S::kConsumers);
-        if (DIRECT) {
+        if (DIRECT) {      // weights are handed over a stage (half a block) at a time: slots 2 (block parity) + half
+            mbar_init(bar(kPpPReady + 2), 2u * S::kConsumers);
+            mbar_init(bar(kPpPReady + 3), 2u * S::kConsumers);
             for (int w = 0; w < 4; ++w) mbar_init(bar(kPpHalves + w), 2u);      // the two warps of 32 rows
         }
         mbar_init(bar(kPpDrain), 1u);
@@ -820,10 +828,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPpThreads, 1) atten
                 }
                 if (j > 0 && ok) {
                     const int i = j - 1;
-                    ok = mbar_wait(bar(kPpPReady + (i & 1)), (uint32_t)((i >> 1) & 1));
+                    if (!DIRECT) ok = mbar_wait(bar(kPpPReady + (i & 1)), (uint32_t)((i >> 1) & 1));
                     const uint32_t a0 = tmem + kPpColS + (uint32_t)S::kKeys * (uint32_t)(i & 1);
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
+                        if (DIRECT) ok = ok && mbar_wait(bar(kPpPReady + 2 * (i & 1) + h), (uint32_t)((i >> 1) & 1));
                         ok = ok && mbar_wait(bar(kPpFullV + (int)vst), vph);
                         if (!ok) break;
                         tc_fence_after();
@@ -1069,8 +1078,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPpThreads, 1) atten
         }
     } else {
         // ======================= consumers: softmax, P, rescale =========================================
-        // DIRECT: two threads a row, of warps w and w + 4, each with one half of a block's keys (one thread a row: 4.2 instead of 3.8 ms for 8 x 2048 tokens after 8192, bound
-        // by what a single warp per scheduler issues).
+        // DIRECT: two threads a row, of warps w and w + 4 (one thread a row: 4.2 instead of 3.8 ms for 8 x 2048 tokens after 8192 in blocks of 64
+        // keys, bound by what a single warp per scheduler issues).
         const int half = DIRECT ? wid >> 2 : 0, crow = tid & (kPpCtaRows - 1);
         const int trow = row0 + crow;
         const int q_off = tok0 + trow / p.gqa;
@@ -1134,7 +1143,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPpThreads, 1) atten
             float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};     // four independent chains
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
-                scores(c + 2 * half, sv[ROT ? 0 : c]);
+                scores(DIRECT ? 2 * c + half : c, sv[ROT ? 0 : c]);
 #pragma unroll
                 for (int i = 0; i < 32; ++i) {
                     if (!SCORED) mx4[i & 3] = fmaxf(mx4[i & 3], sv[ROT ? 0 : c][i]);
@@ -1200,19 +1209,28 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPpThreads, 1) atten
                     lo[i] = pp_pack<FMT>(pa - hf.x, pb - hf.y);
                 }
                 // P takes the place of the scores it came from: value in columns 32 c .. + 15, residual in the next 16
-                tc_st16(t_sj + 32u * (c + 2 * half), hi);
-                tc_st16(t_sj + 32u * (c + 2 * half) + 16u, lo);
+                const uint32_t at = t_sj + 32u * (uint32_t)(DIRECT ? 2 * c + half : c);
+                tc_st16(at, hi);
+                tc_st16(at + 16u, lo);
+                if (DIRECT) {      // the first half's output product runs while the second half's weights are made
+                    tc_wait_st();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive_cluster(leader_pready + 8u * (uint32_t)(2 * (j & 1) + c));
+                }
             }
-            tc_wait_st();
+            if (!DIRECT) tc_wait_st();
             if (SCORED) {
                 const Two sum = add_two(sums[0], sums[1]);
                 ls4[0] = first_of(sum);
                 ls4[1] = second_of(sum);
             }
             l_run = l_run * alpha + ((ls4[0] + ls4[1]) + (ls4[2] + ls4[3]));
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive_cluster(leader_pready + 8u * (uint32_t)(j & 1));
+            if (!DIRECT) {
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive_cluster(leader_pready + 8u * (uint32_t)(j & 1));
+            }
         }
         // the last output product
         if (nblocks > 0 && !aborted_any()) {
