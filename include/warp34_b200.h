@@ -500,7 +500,7 @@ int warp34_qsa_sparse_paged_attn_hadamard_f16(const warp34_exec* ex, const void*
  * key_begin / key_end hold one position per token of the batch: the start of the token's own document in a packed sequence, the end
  * of a prefix that its tokens see whole.  They take any value: a token whose range is empty gets a row of zeros.
  * Everything else is warp34_paged_attention_f16's: batch, masks, strides, scratch (warp34_paged_attention_scored_scratch_bytes for the
- * full grids; less is served more slowly, none by a row-at-a-time fp32 kernel), accuracy, stream, capture.  Masked rows of attn_out are left untouched.
+ * full grids; less is served more slowly, none, where the call needs some, by a row-at-a-time fp32 kernel), accuracy, stream, capture.  Masked rows of attn_out are left untouched.
  * The _FAST_ATTENTION and _TCGEN05_VERIFY flags change nothing here, _PRECISE_ATTENTION selects the fp32 kernel.
  * Layers: _f16 TQ4 (any strides), Q8_0 / FP8 E4M3 (K and V each in either); _bf16 BF16 and TQ4; head_dim 256, 16-token pages; anything else
  * returns cudaErrorNotSupported, and so does a softcap outside [2^-10, 1024] (above, a float is too coarse for the cap itself: 2e-4 of
@@ -527,7 +527,7 @@ size_t warp34_paged_attention_scored_scratch_bytes(const warp34_kv_layer_layout*
  * x of 256 values:
  *   y = x / sqrt(mean(x^2) + rms_eps) * (weight_offset + w)              weight_offset 1: weights stored as w - 1
  *   y[i], y[i + h] <- y[i] cos a - y[i + h] sin a, y[i + h] cos a + y[i] sin a,  a = position * inv_freq[i],  i < h = rotary_dim / 2
- * in fp32 with one rounding at the end; angles are reduced exactly, whatever the position (also negative).  What comes out is what
+ * in fp32 with one rounding at the end; angles are reduced in 64 bits, whatever the position (also negative).  What comes out is what
  * the append of any layer format (warp34_kv_cache_write_strided and its bf16 forms) and the attention entry points take.
  * Rows of q_in hold num_q_heads x 256 values, or, with gate_out, num_q_heads x [256 query | 256 gate]; the gate is copied as it is.
  * position_planes 1: positions[token].  3: positions[plane * position_plane_stride + token], frequency i of plane 1 where i % 3 == 1 and

@@ -153,3 +153,16 @@ def test_in_place_replay_and_streams(env):
         g.replay()
         torch.cuda.synchronize()
     assert torch.equal(q3, qo) and torch.equal(k3, ko)
+
+
+def test_one_row_of_positions_expanded_to_three_planes(env):
+    kv = env
+    q, k, w, pos, inv = _inputs(F16, 4, 2, 19, 64, 1, False, 77)
+    p = pos[0].cuda()
+    outs = []
+    for positions in (p, p.expand(3, 19), p[None].repeat(3, 1)):
+        qo, ko = torch.empty_like(q, memory_format=torch.contiguous_format), torch.empty_like(k, memory_format=torch.contiguous_format)
+        kv.qk_norm_rope(kv.Executor(1 << 12), q, k, w[0], w[1], positions, inv.cuda(), qo, ko, sections=(12, 10, 10))
+        outs.append((qo, ko))
+    for qo, ko in outs[1:]:
+        assert torch.equal(qo, outs[0][0]) and torch.equal(ko, outs[0][1])

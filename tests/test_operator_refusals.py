@@ -145,3 +145,28 @@ def test_scored_attention_wrapper_checks_what_it_is_given(lib):
                    dict(key_begin=torch.zeros(2, dtype=torch.int32)), dict(key_end=torch.zeros(3, dtype=torch.int64))):
         with pytest.raises(ValueError):
             kv.paged_attention_scored(ex, layer, batch, **{**good, **change})
+
+
+def test_tensors_of_the_host_are_refused(lib):
+    """Every argument checked above is right here but for where it lies."""
+    layer = kv.KvLayer(2, 2, device="cpu")
+    batch = kv.StepBatch([0, 3], [0], [3], [[1]], [16, 17, 18], 1, 0.0625, device="cpu")
+    ex = type("E", (), {"ex": ffi.Exec()})()
+    t = lambda *s: torch.zeros(*s, dtype=torch.float16)  # noqa: E731
+    with pytest.raises(ValueError, match="GPU"):
+        kv.paged_attention_scored(ex, layer, batch, t(3, 4, 256), t(3, 4, 256), 4)
+    with pytest.raises(ValueError, match="GPU"):
+        kv.kv_cache_read(ex, layer, batch, t(3, 512), None)
+    with pytest.raises(ValueError, match="GPU"):
+        kv.qk_norm_rope(ex, t(3, 4, 256), None, t(256), None, None, None, t(3, 4, 256), None)
+    with pytest.raises(ValueError, match="GPU"):
+        kv.qk_norm_rope(ex, None, t(3, 2, 256), None, t(256), torch.zeros(3, dtype=torch.int32), torch.zeros(32), None, t(3, 2, 256))
+
+
+def test_a_stride_beyond_the_interface_is_refused(lib):
+    layer = kv.KvLayer(2, 1, device="cpu")
+    batch = kv.StepBatch([0, 2], [0], [2], [[1]], [16, 17], 1, 0.0625, device="cpu")
+    ex = type("E", (), {"ex": ffi.Exec()})()
+    far = torch.empty_strided((2, 256), ((1 << 32) + 256, 1), dtype=torch.float16, device="meta")      # its lower 32 bits are a valid stride
+    with pytest.raises(ValueError, match="stride"):
+        kv.kv_cache_read(ex, layer, batch, far, None)

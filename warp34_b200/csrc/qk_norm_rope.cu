@@ -9,8 +9,8 @@
 // reference's K half with its two roundings, and appends what it makes; this one is for every layer format and the query half.)
 //
 // A head row is a warp: 8 columns a lane, one 16-byte access each way.  Angles: the frequency becomes turns per position as a
-// 64-bit fraction, whose product with the position wraps modulo one turn by itself; what is left is exact to 2^-32 turns at any
-// position (a product in fp32 is off by 2^-7 rad at position 131072).  Sine and cosine are made once per token and block
+// 64-bit fraction, whose product with the position wraps modulo one turn by itself; what is left is off by 2^-32 turns and 2^-52 of the
+// whole angle (a product in fp32 is off by 2^-7 rad at position 131072).  Sine and cosine are made once per token and block
 // (sincospif) and shared by its heads through shared memory, while the rows are on their way.
 //
 // Bound by HBM: 32768 tokens of 24 query heads with gate and 4 key heads (1745 MB) take 268 us, the measured copy rate; without a gate

@@ -496,6 +496,8 @@ def paged_attention_scored(ex, layer, batch, q, out, num_q_heads, softcap=0.0, s
     if key_end is not None:
         _require(key_end.dtype is torch.int32 and key_end.numel() >= n and key_end.is_contiguous(), "key_end: int32, one per token")
         c.key_end = key_end.data_ptr()
+    _require(q.is_cuda and out.is_cuda and (slopes is None or slopes.is_cuda) and (key_begin is None or key_begin.is_cuda) and
+             (key_end is None or key_end.is_cuda), "paged_attention_scored: tensors on the GPU")
     fn = lib.warp34_paged_attention_scored_f16 if dtype == torch.float16 else lib.warp34_paged_attention_scored_bf16
     _check(fn(ex.ex, layer.layout, desc, c, q.data_ptr(), out.data_ptr(), num_q_heads), "warp34_paged_attention_scored")
 
@@ -549,12 +551,18 @@ def qk_norm_rope(ex, q, k, q_weight, k_weight, positions, inv_freq, q_out, k_out
                 not (planes == 1 or (planes == 3 and sections is not None)):
             raise ValueError(f"positions: int32 [{n}], or [3, {n}] and their sections")
         pos, freq, rotary = positions.data_ptr(), inv_freq.data_ptr(), 2 * inv_freq.numel()
+        if planes == 3 and stride[0] == 0 and n > 0:      # one row, expanded
+            planes = 1
         if planes == 3:
             plane, s1, s2 = stride[0], sections[1], sections[2]
+        _require(positions.is_cuda and inv_freq.is_cuda, "positions, inv_freq: on the GPU")
     if valid_token_mask is not None:
         _require(valid_token_mask.dtype is torch.uint8 and valid_token_mask.numel() == n and valid_token_mask.is_contiguous(),
                  "valid_token_mask: uint8, one per token")
         mask = valid_token_mask.data_ptr()
+        _require(valid_token_mask.is_cuda, "valid_token_mask: on the GPU")
+    _require((q is None or (q.is_cuda and q_out.is_cuda and q_weight.is_cuda and (gate_out is None or gate_out.is_cuda))) and
+             (k is None or (k.is_cuda and k_out.is_cuda and k_weight.is_cuda)), "qk_norm_rope: tensors on the GPU")
     a = ffi.QkNormRopeArgs(q_in, k_in, q_to, k_to, gate_to, q_w, k_w, pos, freq, mask, qs, ks, qos, kos, gs, plane,
                            n, hq, hkv, 256, rotary, planes, s1, s2, eps, weight_offset)
     fn = lib.warp34_qk_norm_rope_f16 if dtype is torch.float16 else lib.warp34_qk_norm_rope_bf16
@@ -576,8 +584,10 @@ def kv_cache_read(ex, layer, batch, k_out, v_out, lib=None):
         if len(shape) != 2 or shape[0] < n or shape[1] != cols or stride[1] != 1 or (dtype is not None and t.dtype is not dtype):
             raise ValueError(f"kv_cache_read: outputs of one type, [{n}, {cols}]")
         dtype = t.dtype
-        at += (t.data_ptr(), stride[0] if shape[0] > 1 else max(stride[0], cols))
+        at += (t.data_ptr(), stride[0] if shape[0] > 1 else cols)
     _require(dtype is torch.float16 or dtype is torch.bfloat16, "kv_cache_read: fp16 or bf16 outputs")
+    _require(at[1] < 1 << 31 and at[3] < 1 << 31, "kv_cache_read: a row stride of 2^31 or more")
+    _require((k_out is None or k_out.is_cuda) and (v_out is None or v_out.is_cuda), "kv_cache_read: outputs on the GPU")
     fn = lib.warp34_kv_cache_read_f16 if dtype is torch.float16 else lib.warp34_kv_cache_read_bf16
     _check(fn(ex.ex, layout, desc, at[0], at[2], at[1], at[3]), "warp34_kv_cache_read")
 
