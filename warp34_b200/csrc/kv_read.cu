@@ -71,21 +71,6 @@ __device__ __forceinline__ uint32_t read_half2(float a, float b) {
     const __half2 v = __floats2half2_rn(a, b);
     return *reinterpret_cast<const uint32_t*>(&v);
 }
-// Two numbers in packed arithmetic, each rounded as the scalar instruction does.
-typedef unsigned long long Two;
-__device__ __forceinline__ Two two_of(float a, float b) { return (Two)__float_as_uint(a) | ((Two)__float_as_uint(b) << 32); }
-__device__ __forceinline__ float first_of(Two p) { return __uint_as_float((uint32_t)p); }
-__device__ __forceinline__ float second_of(Two p) { return __uint_as_float((uint32_t)(p >> 32)); }
-__device__ __forceinline__ Two mul_two(Two a, Two b) {
-    Two r;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-__device__ __forceinline__ Two fma_two(Two a, Two b, Two c) {
-    Two r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-    return r;
-}
 // a and b as fp16 pairs of values and of residuals.  The value is cut off, not rounded (one instruction, and exactly what the pair then holds):
 // the residual is below 2^-10 of it and keeps 11 bits of its own.
 __device__ __forceinline__ void read_split(float a, float b, uint32_t& value, uint32_t& residual) {

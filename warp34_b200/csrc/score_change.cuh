@@ -51,26 +51,6 @@ __device__ __forceinline__ float changed_score(const ScoreChange& sc, float t, f
     asm("{\n\t.reg .pred p;\n\tsetp.neu.f32 p, %3, 0f00000000;\n\tselp.f32 %0, %1, %2, p;\n\t}" : "=f"(t) : "f"(capped), "f"(t), "f"(sc.cap));
     return __fmaf_rn(-slope, fabsf(away), t);
 }
-// Two numbers in packed arithmetic, each rounded as the scalar instruction does.
-typedef unsigned long long Two;
-__device__ __forceinline__ Two two_of(float a, float b) { return (Two)__float_as_uint(a) | ((Two)__float_as_uint(b) << 32); }
-__device__ __forceinline__ float first_of(Two p) { return __uint_as_float((uint32_t)p); }
-__device__ __forceinline__ float second_of(Two p) { return __uint_as_float((uint32_t)(p >> 32)); }
-__device__ __forceinline__ Two add_two(Two a, Two b) {
-    Two r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-__device__ __forceinline__ Two mul_two(Two a, Two b) {
-    Two r;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-__device__ __forceinline__ Two fma_two(Two a, Two b, Two c) {
-    Two r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-    return r;
-}
 __device__ __forceinline__ float max_of(float a, float b, float c) {
     float r;
     asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));

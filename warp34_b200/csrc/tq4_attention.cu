@@ -2124,9 +2124,9 @@ static int launch_attention(const warp34_exec* ex, const warp34_kv_layer_layout*
                              ? launch_prefill_pair<WARP34_KV_FORMAT_FP8_E4M3, true>(ex, layout, batch, q_in, attn_out, num_q_heads, io_bf16, og, dev->sm_count, skip_rows, *sc)
                              : launch_prefill_pair<WARP34_KV_FORMAT_Q8_0, true>(ex, layout, batch, q_in, attn_out, num_q_heads, io_bf16, og, dev->sm_count, skip_rows, *sc);
                 } else {
-                rc = layout->k_format == WARP34_KV_FORMAT_FP8_E4M3
-                         ? launch_prefill_pair<WARP34_KV_FORMAT_FP8_E4M3>(ex, layout, batch, q_in, attn_out, num_q_heads, io_bf16, og, dev->sm_count, skip_rows)
-                         : launch_prefill_pair<WARP34_KV_FORMAT_Q8_0>(ex, layout, batch, q_in, attn_out, num_q_heads, io_bf16, og, dev->sm_count, skip_rows);
+                    rc = layout->k_format == WARP34_KV_FORMAT_FP8_E4M3
+                             ? launch_prefill_pair<WARP34_KV_FORMAT_FP8_E4M3>(ex, layout, batch, q_in, attn_out, num_q_heads, io_bf16, og, dev->sm_count, skip_rows)
+                             : launch_prefill_pair<WARP34_KV_FORMAT_Q8_0>(ex, layout, batch, q_in, attn_out, num_q_heads, io_bf16, og, dev->sm_count, skip_rows);
                 }
                 if (rc != 0 || route == kKv8Pair) return rc;
                 const warp34_attention_batch rest = kv8_short_part(batch, num_q_heads / layout->local_kv_heads);

@@ -179,4 +179,25 @@ __device__ __forceinline__ int pool_page(int page, int) { return page; }
 #define W34_BOUNDS_HOST_HOOKS(tag)
 #endif
 
+// Two numbers in packed arithmetic, each rounded as the scalar instruction does.
+typedef unsigned long long Two;
+__device__ __forceinline__ Two two_of(float a, float b) { return (Two)__float_as_uint(a) | ((Two)__float_as_uint(b) << 32); }
+__device__ __forceinline__ float first_of(Two p) { return __uint_as_float((uint32_t)p); }
+__device__ __forceinline__ float second_of(Two p) { return __uint_as_float((uint32_t)(p >> 32)); }
+__device__ __forceinline__ Two add_two(Two a, Two b) {
+    Two r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ Two mul_two(Two a, Two b) {
+    Two r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ Two fma_two(Two a, Two b, Two c) {
+    Two r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+
 }  // namespace w34
