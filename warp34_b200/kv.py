@@ -513,7 +513,7 @@ def _head_rows(t, dtype, n, heads, width, what):
 
 
 def _norm_weight(w, dtype, what):
-    if w.dtype is not dtype or w.shape != (256,) or w.stride() != (1,):
+    if w.dtype is not dtype or w.numel() != 256 or not w.is_contiguous():
         raise ValueError(f"{what}_weight: 256 contiguous values of {dtype}")
     return w.data_ptr()
 
