@@ -584,11 +584,15 @@ static int launch_scored_attention(const warp34_exec* ex, const warp34_kv_layer_
     sc.slopes = change->distance_slopes;
     sc.key_begin = change->key_begin;
     sc.key_end = change->key_end;
-    if ((ex->flags & WARP34_B200_EXEC_FLAG_PRECISE_ATTENTION) == 0 && takes_small(layout, batch, num_q_heads)) {
-        return launch_scored_small(ex, layout, batch, sc, q_in, attn_out, num_q_heads, io_bf16);
+    // The flags that choose among the plain kernels have no builds here.  (The _TCGEN05_VERIFY flag would also send batches of 9 to 24 rows to
+    // the CTA-pair kernel: 682 instead of 357 us for 64 x 4 tokens after 4000 TQ4 keys, 24 / 4 heads.)
+    warp34_exec own = *ex;
+    own.flags &= ~(uint64_t)(WARP34_B200_EXEC_FLAG_FAST_ATTENTION | WARP34_B200_EXEC_FLAG_TCGEN05_VERIFY);
+    if ((own.flags & WARP34_B200_EXEC_FLAG_PRECISE_ATTENTION) == 0 && takes_small(layout, batch, num_q_heads)) {
+        return launch_scored_small(&own, layout, batch, sc, q_in, attn_out, num_q_heads, io_bf16);
     }
-    if (bf16) return launch_bf16_attention(ex, layout, batch, q_in, attn_out, num_q_heads, &sc);
-    return launch_attention(ex, layout, batch, q_in, attn_out, nullptr, num_q_heads, io_bf16, -1, nullptr, &sc);
+    if (bf16) return launch_bf16_attention(&own, layout, batch, q_in, attn_out, num_q_heads, &sc);
+    return launch_attention(&own, layout, batch, q_in, attn_out, nullptr, num_q_heads, io_bf16, -1, nullptr, &sc);
 }
 }  // namespace w34
 
