@@ -1,7 +1,8 @@
-"""Scored attention where its kernels choose by what the call or the cache holds: execution flags that change nothing."""
+"""Scored attention where its kernels choose by what the call or the cache holds: execution flags that change nothing, V rows of any magnitude."""
+import numpy as np
 import pytest
 
-from rows64 import Cache
+from rows64 import Cache, half_step, scored_attention
 
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
@@ -40,3 +41,105 @@ def test_flags_of_the_plain_kernels_change_nothing(env, name, hq, hkv, lens, ctx
         assert ex.ex.flags == flags
     for out in outs[1:]:
         assert torch.equal(outs[0], out)
+
+
+SHARE = {"tq4": 2.0 ** -11, "fp8": 2.0 ** -12, "q8": 2.0 ** -12, "bf16": 2.0 ** -12}      # of sum_k weight_k |V_k|, as test_gpu_scored_attention.py derives it
+
+
+def _check(name, out, want, size, rows=None):
+    got = out.double().cpu().numpy()
+    tol = half_step(want, out.dtype) * (1 + 2.0 ** -8) + SHARE[name] * size
+    with np.errstate(invalid="ignore"):
+        bad = ~(np.abs(got - want) <= tol)
+    if rows is not None:
+        bad = bad & rows
+    assert not bad.any(), f"{name}: {bad.sum()} of {bad.size} outside, worst {np.nanmax(np.abs(got - want) / tol):.2f} x, first {np.argwhere(bad)[0]}"
+
+
+def _microseconds(call):
+    """The fastest of five calls, by the device's clock."""
+    call()
+    times = []
+    for _ in range(5):
+        a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        a.record()
+        call()
+        b.record()
+        torch.cuda.synchronize()
+        times.append(a.elapsed_time(b) * 1e3)
+    return min(times)
+
+
+def _scale_v(cache, powers):
+    """V rows times 2^powers [pages, heads, 16] (whole numbers; never-written rows keep their pattern)."""
+    rows = cache.rows[1]
+    if cache.name == "fp8":
+        d = rows[..., 256:]
+    else:
+        d = rows.reshape(*rows.shape[:3], 4, 68)[..., :4]
+    f = np.ascontiguousarray(d).view(np.float32)
+    f = np.where(np.isfinite(f), f * np.exp2(np.broadcast_to(powers, rows.shape[:3]))[(...,) + (None,) * (f.ndim - 3)], f).astype(np.float32)
+    d[...] = f.view(np.uint8).reshape(d.shape)
+    cache.upload()
+
+
+STREAM = {"decode": (24, 4, [1] * 6, [255, 1, 90, 1000, 47, 48]), "verify": (16, 4, [3, 2, 4, 4, 4, 3], [40, 500, 0, 60, 100, 7])}
+
+
+@pytest.mark.parametrize("power", [-14, -10, 12, "mixed"])
+@pytest.mark.parametrize("shape", list(STREAM))
+@pytest.mark.parametrize("name", ["fp8", "q8"])
+def test_8_bit_values_of_any_magnitude(env, name, shape, power):
+    """V rows far from 1, all of them or each its own way: the share of sum_k weight_k |V_k| that is off does not depend on it."""
+    kv = env["kv"]
+    hq, hkv, lens, ctx = STREAM[shape]
+    cache = Cache(name, hkv, lens, ctx, seed=7, tail=0xff)
+    _scale_v(cache, np.random.default_rng(1).integers(-12, 13, cache.rows[1].shape[:3]) if power == "mixed" else power)
+    q = _queries(name, sum(lens), hq, 8)
+    out = _attend(kv, kv.Executor(64 << 20), cache, cache.batch(), q, hq, softcap=20.0)
+    want, size = scored_attention(cache, q.float().cpu().numpy(), hq, softcap=20.0)
+    _check(name, out, want, size)
+
+
+@pytest.mark.parametrize("name", ["fp8", "q8"])
+def test_8_bit_values_beside_much_larger_ones(env, name):
+    """Drafted tokens of two documents in one group of rows: V rows 2^40 times larger in the one take nothing from the other, and a row of
+    that size with a weight near zero nothing from the rest."""
+    kv = env["kv"]
+    hq, hkv, lens, ctx = 16, 4, [4] * 6, [58, 59, 158, 157, 57, 56]
+    cache = Cache(name, hkv, lens, ctx, seed=9, tail=0xff)
+    pos = np.concatenate([c + np.arange(m) for c, m in zip(ctx, lens)])
+    key_begin = (pos // 60 * 60).astype(np.int32)
+    powers = np.zeros(cache.rows[1].shape[:3], np.int64)
+    for r in range(len(lens)):
+        for k in range(ctx[r] // 60 * 60, min((ctx[r] // 60 + 1) * 60, ctx[r] + lens[r])):      # the document of the request's first new token
+            powers[cache.table[r, k // 16], :, k % 16] = 40
+    _scale_v(cache, powers)
+    q = _queries(name, sum(lens), hq, 10)
+    out = _attend(kv, kv.Executor(64 << 20), cache, cache.batch(), q, hq, softcap=20.0, key_begin=torch.from_numpy(key_begin).cuda())
+    want, size = scored_attention(cache, q.float().cpu().numpy(), hq, softcap=20.0, key_begin=key_begin)
+    small = np.abs(want).max(-1, keepdims=True) < 1e3
+    assert small.any() and not small.all()
+    _check(name, out, want, size, rows=np.broadcast_to(small, want.shape))
+    # one such row, 2000 keys away from a query whose slope leaves it exp(-200)
+    cache = Cache(name, hkv, [1] * 6, [2100] * 6, seed=12, tail=0xff)
+    powers = np.zeros(cache.rows[1].shape[:3], np.int64)
+    powers[cache.table[:, 6], :, 4] = 40      # position 100
+    _scale_v(cache, powers)
+    q, slopes = _queries(name, 6, hq, 13), np.full(hq, 0.1, np.float32)
+    out = _attend(kv, kv.Executor(64 << 20), cache, cache.batch(), q, hq, softcap=20.0, slopes=torch.from_numpy(slopes).cuda())
+    want, size = scored_attention(cache, q.float().cpu().numpy(), hq, softcap=20.0, slopes=slopes)
+    _check(name, out, want, size)
+
+
+@pytest.mark.parametrize("name", ["fp8", "q8"])
+def test_large_8_bit_values_take_no_longer(env, name):
+    kv = env["kv"]
+    hq, hkv, lens, ctx = 16, 4, [1] * 16, [8000] * 16
+    ex, q, times = kv.Executor(64 << 20), _queries(name, 16, hq, 11), []
+    for power in (0, 12):
+        cache = Cache(name, hkv, lens, ctx, seed=10)
+        _scale_v(cache, power)
+        batch, out = cache.batch(), torch.zeros_like(q)
+        times.append(_microseconds(lambda: kv.paged_attention_scored(ex, cache.layer, batch, q, out, hq, softcap=20.0)))
+    assert times[1] < 3 * times[0], times

@@ -322,6 +322,10 @@ __device__ __forceinline__ uint2 lds64_dep(uint32_t addr, uint32_t token) {
     asm("ld.shared.v2.u32 {%0,%1}, [%2+0];  // dep %3" : "=r"(v.x), "=r"(v.y) : "r"(addr), "r"(token));
     return v;
 }
+constexpr float kUpUnset = 7.8886090522101181e-31f, kUpLimit = 32768.0f;      // 2^-100; 2^15
+// 1 / x of a power of two.
+__device__ __forceinline__ float power_inverse(float x) { return __uint_as_float((254u << 23) - __float_as_uint(x)); }
+
 // SPARSE: the query-sparse lists of warp34_qsa_sparse_paged_attn_f16 (see the TQ4 stream kernel): request r
 // is token r, a unit is four entries of its selected list, lanes 0-3 copy their entry's four rows and leave
 // its first position in 16 bytes behind the stage.
@@ -454,6 +458,11 @@ __global__ void __launch_bounds__(kKv8StreamWarps * 32, 1) kv8_attention_stream_
         for (int i = 0; i < 16; ++i) { o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f; }
         float m_run[2] = {-1e30f, -1e30f};
         float l_run[2] = {0.0f, 0.0f};
+        // SCORED: a power of two by which the weights x scales of each of the lane's rows are held, and with them its accumulators, until the
+        // item's end.  It follows the row's own products, so that their residuals stay in fp16's range whatever the magnitude of V (a
+        // scale is about 1/100 of its row's values; with a fixed factor V rows of 2^-10 lost 3e-4 of sum weight |V|, rows above 8000 overflowed),
+        // and rows of another document in the group take nothing from it.  The first page with a key that the row sees sets it.
+        float up[2] = {kUpUnset, kUpUnset}, up_room = kUpLimit / kUpUnset;      // up_room: the largest scale that a weight of 1 may have
 
         const int32_t* blocks = p.batch.block_tables + (size_t)r * p.batch.max_blocks_per_req;
         const uint8_t* k_head_base = (const uint8_t*)(uintptr_t)p.layout.k_base + (size_t)kv_head * p.layout.k_head_stride_bytes;
@@ -672,13 +681,44 @@ __global__ void __launch_bounds__(kKv8StreamWarps * 32, 1) kv8_attention_stream_
             }
             const float mn0 = fmaxf(m_run[0], mx0), mn1 = fmaxf(m_run[1], mx1);
             const bool grew = (mn0 > m_run[0]) || (mn1 > m_run[1]);
-            if (__any_sync(0xffffffffu, grew)) {
-                const float al0 = ex2(m_run[0] - mn0), al1 = ex2(m_run[1] - mn1);
-                l_run[0] *= al0;
-                l_run[1] *= al1;
+            // SCORED: whether a weight of 1 on one of these keys would be held at more than 2^15 (a NaN is passed over: its row ends as one)
+            bool over = false;
+            if (SCORED) {
+                float dv = 0.0f;
+#pragma unroll
+                for (int b = 0; b < NB; ++b) dv = max_of(dv, fabsf(dva[b]), fabsf(dvb[b]));
+                over = dv > up_room;
+            }
+            if (__any_sync(0xffffffffu, grew || over)) {
+                float al[2] = {ex2(m_run[0] - mn0), ex2(m_run[1] - mn1)};
+                l_run[0] *= al[0];
+                l_run[1] *= al[1];
+                if (SCORED) {
+                    const bool first0 = up[0] == kUpUnset && mn0 > -1e29f, first1 = up[1] == kUpUnset && mn1 > -1e29f;
+                    if (__any_sync(0xffffffffu, over || first0 || first1)) {
+#pragma unroll
+                        for (int c = 0; c < 2; ++c) {
+                            float top = 0.0f;      // largest weight x scale of the page's keys
+                            const float wa = msk[c] ? 0.0f : ex2(sc[c] - (c ? mn1 : mn0)), wb = msk[2 + c] ? 0.0f : ex2(sc[2 + c] - (c ? mn1 : mn0));
+#pragma unroll
+                            for (int b = 0; b < NB; ++b) top = fmaxf(top, fmaxf(fabsf(wa * dva[b]), fabsf(wb * dvb[b])));
+#pragma unroll
+                            for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+                            // 2^11 / 2^floor(log2 top): room for scales 16 times larger (60: a zero row, or next to one)
+                            const float fit = __uint_as_float((uint32_t)min(265 - (int)(__float_as_uint(top) >> 23), 127 + 60) << 23);
+                            if (c ? first1 : first0) {
+                                up[c] = fit;      // its accumulators hold zeros
+                            } else if (top * up[c] > kUpLimit) {
+                                al[c] *= fit * power_inverse(up[c]);
+                                up[c] = fit;
+                            }
+                        }
+                        up_room = kUpLimit * power_inverse(fmaxf(up[0], up[1]));
+                    }
+                }
 #pragma unroll
                 for (int t = 0; t < 16; ++t) {
-                    o[t][0] *= al0; o[t][1] *= al1; o[t][2] *= al0; o[t][3] *= al1;
+                    o[t][0] *= al[0]; o[t][1] *= al[1]; o[t][2] *= al[0]; o[t][3] *= al[1];
                 }
                 m_run[0] = mn0;
                 m_run[1] = mn1;
@@ -703,18 +743,17 @@ __global__ void __launch_bounds__(kKv8StreamWarps * 32, 1) kv8_attention_stream_
             }
             l_run[0] += pr[0] + pr[2];
             l_run[1] += pr[1] + pr[3];
-            // P x d_v per scale block as B fragments (k = key, n = query row): fp16 value + fp16 residual
+            // P x d_v per scale block as B fragments (k = key, n = query row): fp16 value + fp16 residual.
+            // SCORED: times a power of two of the row's own (see `up`).
             uint32_t pb[NB][2], pl[NB][2];
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
-                // SCORED: held times kUp, so that the residuals of small weights stay in fp16's range (a scale is about 1/100 of its row's
-                // values; without the factor an output of 0.25 over 317 keys was off by up to 9e-5).  What overflows (V above 60 x 127) ends
-                // non-finite and is computed again.
-                constexpr float kUp = SCORED ? 1024.0f : 1.0f;
-                float pd[4] = {pr[0] * (dva[b] * kUp), pr[1] * (dva[b] * kUp), pr[2] * (dvb[b] * kUp), pr[3] * (dvb[b] * kUp)};
-                if (SCORED && !full) {      // a key that only one of the rows sees: its scales may be NaN to the other
+                float pd[4];
 #pragma unroll
-                    for (int x = 0; x < 4; ++x) if (msk[x]) pd[x] = 0.0f;
+                for (int x = 0; x < 4; ++x) {
+                    const float dv = x < 2 ? dva[b] : dvb[b];
+                    pd[x] = pr[x] * (SCORED ? dv * up[x & 1] : dv);
+                    if (SCORED && !full && msk[x]) pd[x] = 0.0f;      // a key that only one of the rows sees: its scales may be NaN to the other
                 }
 #pragma unroll
                 for (int x = 0; x < 2; ++x) {
@@ -786,6 +825,7 @@ __global__ void __launch_bounds__(kKv8StreamWarps * 32, 1) kv8_attention_stream_
             l_run[0] += __shfl_xor_sync(0xffffffffu, l_run[0], d);
             l_run[1] += __shfl_xor_sync(0xffffffffu, l_run[1], d);
         }
+        const float down[2] = {SCORED ? power_inverse(up[0]) : 1.0f, SCORED ? power_inverse(up[1]) : 1.0f};
         float* stage_o = reinterpret_cast<float*>(ring_gen);   // [8 rows][256]
 #pragma unroll
         for (int mt = 0; mt < 16; ++mt) {
@@ -794,7 +834,7 @@ __global__ void __launch_bounds__(kKv8StreamWarps * 32, 1) kv8_attention_stream_
             const int c = 4 * vw + 2 * (mt & 1);
             if (SCORED) {
 #pragma unroll
-                for (int x = 0; x < 4; ++x) o[mt][x] *= 1.0f / 1024.0f;
+                for (int x = 0; x < 4; ++x) o[mt][x] *= down[x & 1];
             }
             *reinterpret_cast<float2*>(stage_o + (2 * tig) * kHeadDim + c) = make_float2(o[mt][0], o[mt][2]);
             *reinterpret_cast<float2*>(stage_o + (2 * tig + 1) * kHeadDim + c) = make_float2(o[mt][1], o[mt][3]);
