@@ -1,4 +1,5 @@
-"""Scored attention where its kernels choose by what the call or the cache holds: execution flags that change nothing, V rows of any magnitude."""
+"""Scored attention where its kernels choose by what the call or the cache holds: execution flags that change nothing, V rows of any magnitude,
+NaN that a token sees and NaN that it does not."""
 import numpy as np
 import pytest
 
@@ -143,3 +144,65 @@ def test_large_8_bit_values_take_no_longer(env, name):
         batch, out = cache.batch(), torch.zeros_like(q)
         times.append(_microseconds(lambda: kv.paged_attention_scored(ex, cache.layer, batch, q, out, hq, softcap=20.0)))
     assert times[1] < 3 * times[0], times
+
+
+def _spoil_v(cache, r, pos, channels, value=np.nan):
+    """V of every head at `pos` of request r: `value` in the channels (8-bit rows: NaN codes; Q8_0 and TQ4: a scale)."""
+    rows = cache.rows[1][cache.table[r, pos // 16], :, pos % 16]
+    if cache.name == "bf16":
+        rows.view(np.uint16)[:, channels] = 0x7fc0 if np.isnan(value) else 0x7f80
+    elif cache.name == "fp8":
+        rows[:, channels] = 0x7f
+    elif cache.name == "q8":
+        rows[:, 68:72] = np.array([value], np.float32).view(np.uint8)
+    else:
+        rows[:, :2] = np.array([value], np.float16).view(np.uint8)
+
+
+SPOILED = {"decode": (24, 4, [1] * 6, [255, 100, 90, 1000, 47, 48]), "decode_long": (8, 2, [1, 1, 1], [30000, 9000, 40]),
+           "verify": (16, 4, [3, 2, 4, 4, 4, 3], [40, 500, 60, 60, 100, 37]), "chunk": (8, 2, [150, 64, 33], [90, 40, 260]), "chunk_cut": (2, 1, [40], [3000]),
+           "verify_long": (4, 1, [4, 2, 4], [21900, 40, 900])}
+
+
+@pytest.mark.parametrize("shape", list(SPOILED))
+@pytest.mark.parametrize("name", ["tq4", "fp8", "q8", "bf16"])
+def test_channels_without_a_nan_keep_their_results(env, name, shape):
+    """NaN in one channel of a V row of the prefix, which every token sees, and in another channel of a row that only later tokens see: each
+    token is off in the channels of its own keys and in no other (TQ4, whose channels share their scales: in no other token)."""
+    kv = env["kv"]
+    hq, hkv, lens, ctx = SPOILED[shape]
+    cache = Cache(name, hkv, lens, ctx, seed=21, tail=0xff)
+    q = _queries(name, sum(lens), hq, 22)
+    for r in range(len(lens)):
+        if r % 3 != 2 and not (name == "tq4" and len(lens) == 1):      # (some token stays whole)
+            _spoil_v(cache, r, min(37, ctx[r] - 1), [5])
+        if lens[r] > 1:
+            _spoil_v(cache, r, ctx[r] + lens[r] // 2, [9, 200])
+    cache.upload()
+    out = _attend(kv, kv.Executor(64 << 20), cache, cache.batch(), q, hq, softcap=20.0)
+    want, size = scored_attention(cache, q.float().cpu().numpy(), hq, softcap=20.0)
+    finite = np.isfinite(want)
+    assert finite.any() and not finite.all()
+    _check(name, out, want, size, rows=finite)
+    assert torch.isnan(out.cpu()[torch.from_numpy(~finite)]).all()
+
+
+@pytest.mark.parametrize("where", ["prefix", "newest"])
+@pytest.mark.parametrize("name,hq,hkv,lens,ctx", [("bf16", 24, 4, [700], [2048]), ("tq4", 16, 4, [700], [2048]), ("q8", 16, 4, [500, 300], [1000, 40]),
+                                                  ("fp8", 16, 4, [1] * 16, [8000] * 16), ("tq4", 24, 4, [1] * 32, [8000] * 32), ("bf16", 16, 4, [4] * 16, [6000] * 16),
+                                                  ("tq4", 8, 2, [100], [20000])])
+def test_a_nan_that_every_row_sees_is_no_standstill(env, name, hq, hkv, lens, ctx, where):
+    """One NaN in the V of a cached prefix makes every row NaN: such rows are not computed a second time, key by key (which took up to 700 times
+    as long as the call).  What is left is a look at the keys."""
+    kv = env["kv"]
+    cache = Cache(name, hkv, lens, ctx, seed=23)
+    q, batch, ex = _queries(name, sum(lens), hq, 24), cache.batch(), kv.Executor(64 << 20)
+    out = torch.zeros_like(q)
+    call = lambda: kv.paged_attention_scored(ex, cache.layer, batch, q, out, hq, softcap=20.0)  # noqa: E731
+    clean = _microseconds(call)
+    for r in range(len(lens)):
+        _spoil_v(cache, r, 5 if where == "prefix" else ctx[r] - 1, [7])
+    cache.upload()
+    spoiled = _microseconds(call)
+    assert torch.isnan(out).any(-1).all()
+    assert spoiled < 20 * clean, (clean, spoiled)

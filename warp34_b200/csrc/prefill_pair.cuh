@@ -336,9 +336,27 @@ __device__ __forceinline__ void prefill_finish_row(const PrefillPairParams& p, f
     store8(p.attn_out, row_base, lane, p.io_bf16, v);
 }
 
-// The same without a gate, for scored attention: a row that is not finite is computed again by itself.
+// Keys that any of the tokens [tok0, + ntok) of a request can see, by one warp.
+template <bool SCORED>
+__device__ __forceinline__ void prefill_tile_keys(const PrefillPairParams& p, const ReqGeom& g, int tok0, int ntok, int& kv_lo, int& kv_hi) {
+    kv_lo = row_min_kv(p.batch, g, tok0);      // (both limits grow with the token)
+    kv_hi = row_max_kv(p.batch, g, tok0 + ntok - 1);
+    if (SCORED && (p.sc.key_begin != nullptr || p.sc.key_end != nullptr)) {      // limits of the tokens' own: in no order
+        int lo = 0x7fffffff, hi = -1;
+        for (int t = tok0 + (int)(threadIdx.x & 31); t < tok0 + ntok; t += 32) {
+            if (p.batch.valid_token_mask != nullptr && p.batch.valid_token_mask[g.q_start + t] == 0) continue;
+            const int first = row_first_key<true>(p.batch, p.sc, g, t), last = row_last_key<true>(p.batch, p.sc, g, t);
+            if (first <= last) { lo = min(lo, first); hi = max(hi, last); }
+        }
+        kv_lo = __reduce_min_sync(0xffffffffu, lo);
+        kv_hi = __reduce_max_sync(0xffffffffu, hi);
+    }
+}
+
+// Scored attention, a row from the sum of its keys' parts, by one warp: normalised, in the natural basis, stored.  A row that is not finite
+// is computed again by itself, unless its own keys explain it; `whole`: it was.
 template <bool ROT>
-__device__ __forceinline__ void prefill_finish_scored_row(const PrefillPairParams& p, float (&v)[8], float l, int req, int q_off, int q_head, int lane) {
+__device__ __forceinline__ void prefill_finish_scored_row(const PrefillPairParams& p, float (&v)[8], float l, int req, int q_off, int q_head, int lane, bool whole) {
     const float inv = l != 0.0f ? 1.0f / (ROT ? l * (kPpLutScale * 16.0f) : l) : 0.0f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] *= inv;
@@ -349,11 +367,17 @@ __device__ __forceinline__ void prefill_finish_scored_row(const PrefillPairParam
     bool fine = is_finite(l);
 #pragma unroll
     for (int i = 0; i < 8; ++i) fine = fine && is_finite(v[i]);
-    if (!__all_sync(0xffffffffu, fine)) {
-        const ScoredRow one = {&p.layout, &p.batch, &p.sc, p.q_in, p.io_bf16, p.num_q_heads, p.gqa};
-        scored_row_whole(one, req, q_off, q_head, v);
-    }
     store8(p.attn_out, ((size_t)(p.batch.query_start_loc[req] + q_off) * p.num_q_heads + q_head) * kHeadDim, lane, p.io_bf16, v);
+    if (!whole && !__all_sync(0xffffffffu, fine)) {
+        const ScoredRow one = {&p.layout, &p.batch, &p.sc, p.q_in, p.io_bf16, p.num_q_heads, p.gqa};
+        const ReqGeom g = load_req(p.batch, req);
+        const int tok0 = q_off - q_off % p.tok_per_tile;
+        int lo, hi;
+        prefill_tile_keys<true>(p, g, tok0, min(p.tok_per_tile, g.q_len - tok0), lo, hi);
+        if (!scored_bad_rows_call(one, req, q_head / p.gqa, lo, hi, 0, 1).explains(row_first_key<true>(p.batch, p.sc, g, q_off), row_last_key<true>(p.batch, p.sc, g, q_off))) {
+            scored_row_whole_call(one, req, q_off, q_head, p.attn_out);
+        }
+    }
 }
 
 // One query row over its keys in [lo, hi] in fp32 by one warp, as the attention kernel leaves it (columns [8 lane, + 8) of the accumulator,
@@ -456,7 +480,7 @@ __global__ void __launch_bounds__(128) prefill_merge_kernel(const __grid_constan
         v[0] += ws * a.x; v[1] += ws * a.y; v[2] += ws * a.z; v[3] += ws * a.w;
         v[4] += ws * b.x; v[5] += ws * b.y; v[6] += ws * b.z; v[7] += ws * b.w;
     }
-    if constexpr (SCORED) prefill_finish_scored_row<ROT>(p, v, l_tot, r, tok - p.batch.query_start_loc[r], (int)(row % p.num_q_heads), lane);
+    if constexpr (SCORED) prefill_finish_scored_row<ROT>(p, v, l_tot, r, tok - p.batch.query_start_loc[r], (int)(row % p.num_q_heads), lane, false);
     else prefill_finish_row<ROT>(p, v, l_tot, (size_t)row * kHeadDim, lane);
 }
 
@@ -592,19 +616,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPpThreads, 1) atten
     const int ntok = min(tpt, g.q_len - tok0);
     const int rows_used = ntok * p.gqa;
     const int row0 = (int)rank * kPpCtaRows;      // first row of this CTA in the tile
-    // keys any row of the pair can see (both limits grow with the token)
-    int kv_lo = row_min_kv(p.batch, g, tok0);
-    int kv_hi = row_max_kv(p.batch, g, tok0 + ntok - 1);
-    if (SCORED && (p.sc.key_begin != nullptr || p.sc.key_end != nullptr)) {      // limits of the tokens' own: in no order
-        int lo = 0x7fffffff, hi = -1;
-        for (int t = tok0 + lane; t < tok0 + ntok; t += 32) {
-            if (p.batch.valid_token_mask != nullptr && p.batch.valid_token_mask[g.q_start + t] == 0) continue;
-            const int first = row_first_key<true>(p.batch, p.sc, g, t), last = row_last_key<true>(p.batch, p.sc, g, t);
-            if (first <= last) { lo = min(lo, first); hi = max(hi, last); }
-        }
-        kv_lo = __reduce_min_sync(0xffffffffu, lo);
-        kv_hi = __reduce_max_sync(0xffffffffu, hi);
-    }
+    // keys any row of the pair can see
+    int kv_lo, kv_hi;
+    prefill_tile_keys<SCORED>(p, g, tok0, ntok, kv_lo, kv_hi);
     const bool any_keys = kv_hi >= kv_lo;
     const int pg_lo = any_keys ? (kv_lo >> 4) : 0, pg_hi = any_keys ? (kv_hi >> 4) : -1;
     const int all_lo = any_keys ? (kv_lo >> KB) : 0, all = any_keys ? ((kv_hi >> KB) - all_lo + 1) : 0;
@@ -1272,6 +1286,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPpThreads, 1) atten
     }
     tc_fence_before();
     __syncthreads();
+    uint32_t again = 0u;      // SCORED: rows that are not finite, four bits for each of the warp's groups
     if (!aborted) {
         const int first_token = place[2], rows = place[3], q_start = place[4];
         const bool by_rows = !fits || p.splits > 1;      // (tiles that are computed in fp32, and parts of a tile's keys, which are not rotated here)
@@ -1318,7 +1333,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPpThreads, 1) atten
                     if (lane == 0) p.parts_ml[part_row] = make_float2(m, l);
                     continue;
                 }
-                if constexpr (SCORED) prefill_finish_scored_row<ROT>(p, v, l, place[0], q_off, q_head, lane);
+                if constexpr (SCORED) prefill_finish_scored_row<ROT>(p, v, l, place[0], q_off, q_head, lane, true);      // (one range of keys: computed in fp32)
                 else prefill_finish_row<ROT>(p, v, l, out_row * kHeadDim, lane);
             }
         } else {
@@ -1358,12 +1373,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPpThreads, 1) atten
                 }
                 if (ROT) rotate_registers<4 + 8 + 16>(v);
                 const uint32_t signs = ROT ? chunk_signs(j) : 0u;
-                uint32_t again = 0u;      // SCORED: lanes of rows that are not finite
                 if (SCORED) {
                     bool fine = is_finite(l);
 #pragma unroll
                     for (int k = 0; k < 32; ++k) fine = fine && is_finite(v[k]);
-                    again = __ballot_sync(0xffffffffu, ok && !fine);
+                    const uint32_t odd = __ballot_sync(0xffffffffu, ok && !fine);
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) again |= ((odd >> (8 * q)) & 0xffu) != 0u ? 1u << (4 * (grp / kPpWarps) + q) : 0u;
                 }
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
@@ -1374,23 +1390,33 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPpThreads, 1) atten
                     if (i < 2 && gated) load8_raw(p.og.gate, out_base, j + 8 * (i + 2), gate[i & 1]);
                     if (ok) store8(p.attn_out, out_base, j + 8 * i, p.io_bf16, x);
                 }
-                if (SCORED && again != 0u) {
-                    __syncwarp();      // the rows that follow overwrite what was just stored
-#pragma unroll 1
-                    for (int q = 0; q < 4; ++q) {
-                        if (((again >> (8 * q)) & 0xffu) == 0u) continue;
-                        const int r = (int)cluster_rank() * kPpCtaRows + 4 * grp + q;
-                        const int off = first_token + r / p.gqa, head = kv_head * p.gqa + r % p.gqa;
-                        const ScoredRow one = {&p.layout, &p.batch, &p.sc, p.q_in, p.io_bf16, p.num_q_heads, p.gqa};
-                        float y[8];
-                        scored_row_whole(one, place[0], off, head, y);
-                        store8(p.attn_out, ((size_t)(q_start + off) * p.num_q_heads + head) * kHeadDim, lane, p.io_bf16, y);
-                    }
-                }
             }
         }
     } else if (tid == 0 && p.status != nullptr) {
         atomicOr(p.status, 1);
+    }
+    if constexpr (SCORED) {      // a second look at rows that are not finite (scored_rows.cuh); every thread of the CTA comes here, after an abort as well
+        int* bad_k = reinterpret_cast<int*>(gen + S::kOffBars + S::kWords + 24);
+        int* bad_v = reinterpret_cast<int*>(gen + S::kOffBars + S::kWords + 52);
+        if (tid < 2) bad_k[tid] = bad_v[tid] = tid == 0 ? 0x7fffffff : -1;
+        if (__syncthreads_or(again != 0u)) {
+            const ScoredRow one = {&p.layout, &p.batch, &p.sc, p.q_in, p.io_bf16, p.num_q_heads, p.gqa};
+            const ReqGeom g = load_req(p.batch, place[0]);
+            const int first_token = place[2];
+            int lo, hi;
+            prefill_tile_keys<true>(p, g, first_token, place[3] / p.gqa, lo, hi);
+            scored_bad_join(scored_bad_rows_call(one, place[0], kv_head, lo, hi, wid, kPpWarps), bad_k, bad_v);
+            __syncthreads();
+            ScoredBad bad;
+            bad.k_first = bad_k[0]; bad.k_last = bad_k[1]; bad.v_first = bad_v[0]; bad.v_last = bad_v[1];
+            for (; again != 0u; again &= again - 1u) {
+                const int bit = __ffs((int)again) - 1;
+                const int r = (int)cluster_rank() * kPpCtaRows + 4 * (wid + kPpWarps * (bit >> 2)) + (bit & 3);
+                const int off = first_token + r / p.gqa, head = kv_head * p.gqa + r % p.gqa;
+                if (bad.explains(row_first_key<true>(p.batch, p.sc, g, off), row_last_key<true>(p.batch, p.sc, g, off))) continue;
+                scored_row_whole_call(one, place[0], off, head, p.attn_out);
+            }
+        }
     }
     // neither CTA leaves (or frees tensor memory) while the other may still signal it
     cluster_sync_all();

@@ -2,7 +2,9 @@
 // tensor-core kernels do not take (no workspace, other packings, mixed 8-bit formats, WARP34_B200_EXEC_FLAG_PRECISE_ATTENTION), and the
 // second look at rows that came out non-finite.  The latter because a product of a tile's weights with its V rows meets every row of
 // the tile with every key of it: a NaN or infinity in the V of a key that one row must not see (another document's, say) is 0 x NaN there.
-// A row that has such a key in sight comes out non-finite again.
+// A row that sees every such key itself is what it must be, and is left alone (scored_bad_rows: one look at the keys of its tile, bound by
+// memory.  Computing such rows again, key by key, took 1000 times as long as the call: 74 ms for 2048 BF16 tokens after 2048, 24 / 4 heads,
+// behind one NaN in the prefix).
 // Included by tq4_attention.cu.
 #pragma once
 
@@ -104,21 +106,179 @@ __device__ __forceinline__ void scored_row_keys(const ScoredRow& p, int req, int
 #pragma unroll
             for (int i = 0; i < 8; ++i) acc[i] = __fmaf_rn(acc[i], alpha, w * x[i]);
         }
+        if (l != l) return;      // a NaN in the query or in a key: the row is NaN whatever follows
     }
 }
 
-// The same for all of a row's keys, normalised and in the natural basis.
-__device__ __forceinline__ void scored_row_whole(const ScoredRow& p, int req, int q_off, int q_head, float (&v)[8]) {
-    float m, l;
+// Keys whose rows reach every row that sees them: K rows with a NaN, V rows with a NaN or infinity.  First and last position (none: first > last).
+struct ScoredBad {
+    int k_first = 0x7fffffff, k_last = -1, v_first = 0x7fffffff, v_last = -1;
+    // Whether a row that sees keys [lo, hi], of a tile whose keys this is about, is non-finite of its own: it sees such a key, and no V row it
+    // does not see can have reached it.  (Where neither holds, an operand has left the range of the tensor cores' type.)
+    __device__ __forceinline__ bool explains(int lo, int hi) const {
+        const bool v = v_first <= v_last;
+        if (v && (v_first < lo || v_last > hi)) return false;
+        return (v && lo <= hi) || (k_first >= lo && k_first <= hi) || (k_last >= lo && k_last <= hi);
+    }
+};
+
+// The 16 rows of a (page, head) in canonical packing: the lane's part of a bit for each that holds a NaN or, with INFINITIES, an infinity.  A
+// lane looks at scales (TQ4, Q8_0), at scales and eight codes of every row (FP8), or at 16 bytes of every row (BF16).
+template <bool INFINITIES>
+__device__ __forceinline__ uint32_t scored_bad_scales(const uint8_t* run, size_t token_stride, int format, int lane) {
+    constexpr uint32_t f16 = INFINITIES ? 0x7bffu : 0x7c00u, f32 = INFINITIES ? 0x7f7fffffu : 0x7f800000u;
+    if (format == WARP34_KV_FORMAT_TQ4) {
+        const uint32_t d = *reinterpret_cast<const uint16_t*>(run + (size_t)(lane >> 1) * token_stride + kTq4BlockBytes * (lane & 1));
+        return ((d & 0x7fffu) > f16 ? 1u : 0u) << (lane >> 1);
+    }
+    if (format == WARP34_KV_FORMAT_FP8_E4M3) {
+        const uint32_t d = *reinterpret_cast<const uint32_t*>(run + (size_t)(lane >> 1) * token_stride + kHeadDim + 4 * (lane & 1));
+        return ((d & 0x7fffffffu) > f32 ? 1u : 0u) << (lane >> 1);
+    }
+    uint32_t bad = 0u;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int t = (lane >> 2) + 8 * i;
+        const uint32_t d = *reinterpret_cast<const uint32_t*>(run + (size_t)t * token_stride + 68 * (lane & 3));
+        bad |= ((d & 0x7fffffffu) > f32 ? 1u : 0u) << t;
+    }
+    return bad;
+}
+template <bool INFINITIES>
+__device__ __forceinline__ uint32_t scored_bad_elements(const uint8_t* run, size_t token_stride, int format, int lane) {
+    constexpr uint32_t b16 = INFINITIES ? 0x7f7fu : 0x7f80u;
+    uint32_t bad = 0u;
+    if (format == WARP34_KV_FORMAT_BF16) {
+#pragma unroll 2
+        for (int t = 0; t < 16; ++t) {
+            const uint4 w = *reinterpret_cast<const uint4*>(run + (size_t)t * token_stride + 16 * lane);
+            const uint32_t x[4] = {w.x, w.y, w.z, w.w};
+            bool any = false;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) any = any || (x[i] & 0x7fffu) > b16 || ((x[i] >> 16) & 0x7fffu) > b16;
+            bad |= (any ? 1u : 0u) << t;
+        }
+        return bad;
+    }
+#pragma unroll 4
+    for (int t = 0; t < 16; ++t) {      // the code 0x7f, of either sign, is NaN
+        const uint2 w = *reinterpret_cast<const uint2*>(run + (size_t)t * token_stride + 8 * lane);
+        const uint32_t any = (((w.x & 0x7f7f7f7fu) + 0x01010101u) | ((w.y & 0x7f7f7f7fu) + 0x01010101u)) & 0x80808080u;
+        bad |= (any != 0u ? 1u : 0u) << t;
+    }
+    return bad | scored_bad_scales<INFINITIES>(run, token_stride, format, lane);
+}
+
+// The keys [lo, hi] of one kv head, every `step`th page from the `first` on, by one warp.  K and V have one format.
+__device__ __forceinline__ ScoredBad scored_bad_rows(const ScoredRow& p, int req, int kv_head, int lo, int hi, int first, int step) {
+    const int lane = threadIdx.x & 31;
+    const warp34_attention_batch& b = *p.batch;
+    const warp34_kv_layer_layout& lay = *p.layout;
+    const int32_t* blocks = b.block_tables + (size_t)req * b.max_blocks_per_req;
+    const uint8_t* k_head = (const uint8_t*)(uintptr_t)lay.k_base + (size_t)kv_head * lay.k_head_stride_bytes;
+    const uint8_t* v_head = (const uint8_t*)(uintptr_t)lay.v_base + (size_t)kv_head * lay.v_head_stride_bytes;
+    const int format = lay.k_format;
+    ScoredBad res;
+    if (lo > hi) return res;
+    const int last = hi >> 4;
+    auto take = [&](int pg, uint32_t k, uint32_t v) {
+        const int pos = pg << 4;
+        const uint32_t in = (0xffffu << max(lo - pos, 0)) & (0xffffu >> max(pos + 15 - hi, 0));
+        k = __reduce_or_sync(0xffffffffu, k) & in;
+        v = __reduce_or_sync(0xffffffffu, v) & in;
+        if (k != 0u) {
+            res.k_first = min(res.k_first, pos + __ffs((int)k) - 1);
+            res.k_last = max(res.k_last, pos + 31 - __clz((int)k));
+        }
+        if (v != 0u) {
+            res.v_first = min(res.v_first, pos + __ffs((int)v) - 1);
+            res.v_last = max(res.v_last, pos + 31 - __clz((int)v));
+        }
+    };
+    for (int pg0 = (lo >> 4) + first; pg0 <= last; pg0 += 32 * step) {
+        const int mine = pg0 + lane * step;      // a lane per page of the table
+        const int32_t ids = mine <= last ? block_table_page(blocks, mine, b.max_blocks_per_req, kInScalar) : 0;
+        const int n = min((last - pg0) / step + 1, 32);
+        if (format == WARP34_KV_FORMAT_BF16 || format == WARP34_KV_FORMAT_FP8_E4M3) {
+#pragma unroll 1
+            for (int i = 0; i < n; ++i) {
+                const size_t id = (size_t)__shfl_sync(0xffffffffu, ids, i);
+                take(pg0 + i * step, scored_bad_elements<false>(k_head + id * lay.k_page_stride_bytes, lay.k_token_stride_bytes, format, lane),
+                     scored_bad_elements<true>(v_head + id * lay.v_page_stride_bytes, lay.v_token_stride_bytes, format, lane));
+            }
+            continue;
+        }
+#pragma unroll 1
+        for (int i0 = 0; i0 < n; i0 += 4) {      // four pages on their way at once
+            uint32_t k[4], v[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const size_t id = (size_t)__shfl_sync(0xffffffffu, ids, min(i0 + i, n - 1));
+                k[i] = scored_bad_scales<false>(k_head + id * lay.k_page_stride_bytes, lay.k_token_stride_bytes, format, lane);
+                v[i] = scored_bad_scales<true>(v_head + id * lay.v_page_stride_bytes, lay.v_token_stride_bytes, format, lane);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) take(pg0 + min(i0 + i, n - 1) * step, k[i], v[i]);
+        }
+    }
+    return res;
+}
+
+// Joins what a block's warps found: k and v hold {INT_MAX, -1} before, and the block meets at a barrier on either side.
+__device__ __forceinline__ void scored_bad_join(const ScoredBad& mine, int* k, int* v) {
+    if ((threadIdx.x & 31) != 0) return;
+    if (mine.k_first <= mine.k_last) { atomicMin(&k[0], mine.k_first); atomicMax(&k[1], mine.k_last); }
+    if (mine.v_first <= mine.v_last) { atomicMin(&v[0], mine.v_first); atomicMax(&v[1], mine.v_last); }
+}
+
+// The states of W warps over parts of a row's keys (columns, maximum, mass; a mass of 0: no keys) -> the row, by one warp.
+template <int W>
+__device__ __forceinline__ void scored_row_join(float (*s_acc)[kHeadDim], const float* s_m, const float* s_l, bool rotated, float (&acc)[8]) {
+    const int lane = threadIdx.x & 31;
+    float m_tot = s_m[0], l_tot = 0.0f;
+#pragma unroll 4
+    for (int w = 1; w < W; ++w) m_tot = fmaxf(m_tot, s_m[w]);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) acc[i] = 0.0f;
+#pragma unroll 4
+    for (int w = 0; w < W; ++w) {
+        if (s_l[w] == 0.0f) continue;      // no keys
+        const float wgt = ex2(s_m[w] - m_tot);
+        l_tot += s_l[w] * wgt;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) acc[i] += s_acc[w][8 * lane + i] * wgt;
+    }
+    const float inv = l_tot == 0.0f ? 0.0f : 1.0f / l_tot;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) acc[i] *= rotated ? inv * 0.0625f : inv;
+    if (rotated) {
+        butterfly8<5>(acc, lane);
+        sign8(acc, lane);
+    }
+}
+
+// The same for all of a row's keys: normalised, in the natural basis, stored at `out`.
+__device__ __forceinline__ void scored_row_whole(const ScoredRow& p, int req, int q_off, int q_head, void* out) {
+    const int lane = threadIdx.x & 31;
+    float v[8], m, l;
     scored_row_keys(p, req, q_off, q_head, 0, 0x7ffffffe, 0, 1, v, m, l);
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     const bool rotated = p.layout->v_format == WARP34_KV_FORMAT_TQ4;
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] *= rotated ? inv * 0.0625f : inv;
     if (rotated) {
-        butterfly8<5>(v, threadIdx.x & 31);
-        sign8(v, threadIdx.x & 31);
+        butterfly8<5>(v, lane);
+        sign8(v, lane);
     }
+    store8(out, ((size_t)(p.batch->query_start_loc[req] + q_off) * p.num_q_heads + q_head) * kHeadDim, lane, p.io_bf16, v);
+}
+
+// Both as calls, for the chunk kernel: in line they take registers from what is around them.
+__device__ __noinline__ ScoredBad scored_bad_rows_call(const ScoredRow p, int req, int kv_head, int lo, int hi, int first, int step) {
+    return scored_bad_rows(p, req, kv_head, lo, hi, first, step);
+}
+__device__ __noinline__ void scored_row_whole_call(const ScoredRow p, int req, int q_off, int q_head, void* out) {
+    scored_row_whole(p, req, q_off, q_head, out);
 }
 
 // One block of four warps per (token, q head); warp w takes the keys first + w, + 4, ...
@@ -148,26 +308,7 @@ __global__ void __launch_bounds__(128) scored_rows_kernel(const __grid_constant_
     if (lane == 0) { s_m[wid] = m; s_l[wid] = l; }
     __syncthreads();
     if (wid != 0) return;
-    const float m_tot = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3]));
-    float l_tot = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) acc[i] = 0.0f;
-#pragma unroll
-    for (int w = 0; w < 4; ++w) {
-        if (s_l[w] == 0.0f) continue;      // no keys
-        const float wgt = ex2(s_m[w] - m_tot);
-        l_tot += s_l[w] * wgt;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) acc[i] += s_acc[w][8 * lane + i] * wgt;
-    }
-    const bool rotated = p.layout.v_format == WARP34_KV_FORMAT_TQ4;
-    const float inv = l_tot == 0.0f ? 0.0f : 1.0f / l_tot;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) acc[i] *= rotated ? inv * 0.0625f : inv;
-    if (rotated) {
-        butterfly8<5>(acc, lane);
-        sign8(acc, lane);
-    }
+    scored_row_join<4>(s_acc, s_m, s_l, p.layout.v_format == WARP34_KV_FORMAT_TQ4, acc);
     store8(p.attn_out, ((size_t)tok * p.num_q_heads + q_head) * kHeadDim, lane, p.io_bf16, acc);
 }
 

@@ -1409,11 +1409,13 @@ constexpr int kRowTripleFloats = kHeadDim + 2;
 // either normalise + inverse rotation + fp16 store, or (PARTIAL_OUT) store the merged
 // (acc, m, l) triple for a cross-shard merge.  MW = 4 for batches; a long single sequence has
 // hundreds of partials per row and only a few rows, for which MW = 32.
-// SCORED: a state that is not finite is kept, and a row that ends so is computed again by itself (scored_rows.cuh).
+// SCORED: a state that is not finite is kept, and a row that ends so without a key of its own to explain it is computed again by itself
+// (scored_rows.cuh), by the block's warps together.
 template <bool PARTIAL_OUT, int MW, bool SCORED = false>
-__global__ void __launch_bounds__(MW * 32) tq4_attention_merge_kernel(const __grid_constant__ StreamParams p) {
+__global__ void __launch_bounds__(MW * 32, SCORED && MW == 4 ? 7 : 0) tq4_attention_merge_kernel(const __grid_constant__ StreamParams p) {
     __shared__ __align__(16) float s_acc[MW][kHeadDim];
     __shared__ float s_m[MW], s_l[MW];
+    __shared__ int s_again[SCORED ? 5 : 1];      // SCORED: whether the row is not finite; K, V positions (ScoredBad)
     grid_dependency_wait();
     grid_launch_dependents();
     const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
@@ -1533,49 +1535,76 @@ __global__ void __launch_bounds__(MW * 32) tq4_attention_merge_kernel(const __gr
     if (SCORED) odd = __any_sync(0xffffffffu, odd);
     if (lane == 0) { s_m[wid] = m_tot; s_l[wid] = SCORED && odd ? __uint_as_float(0x7fc00000u) : l_tot; }
     __syncthreads();
-    if (wid != 0) return;
-    m_tot = s_m[0];
-#pragma unroll
-    for (int w = 1; w < MW; ++w) m_tot = fmaxf(m_tot, s_m[w]);
-    l_tot = 0.0f;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) acc[j] = 0.0f;
-#pragma unroll 4
-    for (int w = 0; w < MW; ++w) {
-        const float wgt = (s_l[w] > 0.0f) ? ex2(s_m[w] - m_tot) : 0.0f;
-        l_tot += s_l[w] * wgt;      // (SCORED: a mass that is NaN makes the sum NaN with any weight)
-        const float4 a = *reinterpret_cast<const float4*>(&s_acc[w][8 * lane]), b = *reinterpret_cast<const float4*>(&s_acc[w][8 * lane + 4]);
-        acc[0] += a.x * wgt; acc[1] += a.y * wgt; acc[2] += a.z * wgt; acc[3] += a.w * wgt;
-        acc[4] += b.x * wgt; acc[5] += b.y * wgt; acc[6] += b.z * wgt; acc[7] += b.w * wgt;
-    }
-    if (PARTIAL_OUT) {
-        float* dst = p.triple_out + ((size_t)tok * p.num_q_heads + q_head) * kRowTripleFloats;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) dst[8 * lane + j] = acc[j];
-        if (lane == 0) { dst[kHeadDim] = m_tot; dst[kHeadDim + 1] = l_tot; }
-        return;
-    }
+    if (!SCORED && wid != 0) return;
     const size_t out_base = ((size_t)tok * p.num_q_heads + q_head) * kHeadDim;
-    const float inv = (l_tot > 0.0f) ? (1.0f / (p.natural ? l_tot : l_tot * (kLutScale * 16.0f))) : 0.0f;
+    if (!SCORED || wid == 0) {
+        m_tot = s_m[0];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) acc[j] *= inv;
-    if (!p.natural) {
-        butterfly8<5>(acc, lane);
-        sign8(acc, lane);
-    }
-    if (SCORED) {
-        bool fine = is_finite(l_tot);
+        for (int w = 1; w < MW; ++w) m_tot = fmaxf(m_tot, s_m[w]);
+        l_tot = 0.0f;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) fine = fine && is_finite(acc[j]);
-        if (!__all_sync(0xffffffffu, fine)) {
-            const ScoredRow row = {&p.layout, &p.batch, &p.sc, p.q_in, p.io_bf16, p.num_q_heads, p.gqa};
-            scored_row_whole(row, r, tok - p.batch.query_start_loc[r], q_head, acc);
+        for (int j = 0; j < 8; ++j) acc[j] = 0.0f;
+#pragma unroll 4
+        for (int w = 0; w < MW; ++w) {
+            const float wgt = (s_l[w] > 0.0f) ? ex2(s_m[w] - m_tot) : 0.0f;
+            l_tot += s_l[w] * wgt;      // (SCORED: a mass that is NaN makes the sum NaN with any weight)
+            const float4 a = *reinterpret_cast<const float4*>(&s_acc[w][8 * lane]), b = *reinterpret_cast<const float4*>(&s_acc[w][8 * lane + 4]);
+            acc[0] += a.x * wgt; acc[1] += a.y * wgt; acc[2] += a.z * wgt; acc[3] += a.w * wgt;
+            acc[4] += b.x * wgt; acc[5] += b.y * wgt; acc[6] += b.z * wgt; acc[7] += b.w * wgt;
+        }
+        if (PARTIAL_OUT) {
+            float* dst = p.triple_out + ((size_t)tok * p.num_q_heads + q_head) * kRowTripleFloats;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) dst[8 * lane + j] = acc[j];
+            if (lane == 0) { dst[kHeadDim] = m_tot; dst[kHeadDim + 1] = l_tot; }
+            return;
+        }
+        const float inv = (l_tot > 0.0f) ? (1.0f / (p.natural ? l_tot : l_tot * (kLutScale * 16.0f))) : 0.0f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) acc[j] *= inv;
+        if (!p.natural) {
+            butterfly8<5>(acc, lane);
+            sign8(acc, lane);
         }
     }
-    uint32_t gate[4];
-    load_gate8(p.og, out_base, lane, gate);
-    apply_output_gate8(acc, p.og, gate, lane, p.io_bf16);
-    store8(p.attn_out, out_base, lane, p.io_bf16, acc);
+    if constexpr (SCORED) {      // (no gate; the second look stands behind the exit of a row that needs none, in front of it its code made a call 1 us longer)
+        if (wid == 0) {
+            bool fine = is_finite(l_tot);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) fine = fine && is_finite(acc[j]);
+            fine = __all_sync(0xffffffffu, fine);
+            if (!fine && !is_finite(l_tot)) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) acc[j] = __uint_as_float(0x7fc00000u);
+            }
+            store8(p.attn_out, out_base, lane, p.io_bf16, acc);
+            if (lane < 5) s_again[lane] = lane == 0 ? !fine : (lane & 1) ? 0x7fffffff : -1;
+        }
+        __syncthreads();
+        if (__builtin_expect(s_again[0] == 0, 1)) return;      // block-uniform
+        const ScoredRow row = {&p.layout, &p.batch, &p.sc, p.q_in, p.io_bf16, p.num_q_heads, p.gqa};
+        const int lo = plan_array(p.scratch, 2, R)[r] << 4, hi = min(lo + (npages << 4), p.batch.seq_lens_after[r]) - 1;
+        scored_bad_join(scored_bad_rows(row, r, kv_head, lo, hi, wid, MW), s_again + 1, s_again + 3);
+        __syncthreads();
+        const ReqGeom g = load_req(p.batch, r);
+        ScoredBad bad;
+        bad.k_first = s_again[1]; bad.k_last = s_again[2]; bad.v_first = s_again[3]; bad.v_last = s_again[4];
+        if (bad.explains(row_first_key<true>(p.batch, p.sc, g, tok - g.q_start), row_last_key<true>(p.batch, p.sc, g, tok - g.q_start))) return;
+        float m, l;
+        scored_row_keys(row, r, tok - g.q_start, q_head, 0, 0x7ffffffe, wid, MW, acc, m, l);
+        *reinterpret_cast<float4*>(&s_acc[wid][8 * lane]) = make_float4(acc[0], acc[1], acc[2], acc[3]);
+        *reinterpret_cast<float4*>(&s_acc[wid][8 * lane + 4]) = make_float4(acc[4], acc[5], acc[6], acc[7]);
+        if (lane == 0) { s_m[wid] = m; s_l[wid] = l; }
+        __syncthreads();
+        if (wid != 0) return;
+        scored_row_join<MW>(s_acc, s_m, s_l, !p.natural, acc);
+        store8(p.attn_out, out_base, lane, p.io_bf16, acc);
+    } else {
+        uint32_t gate[4];
+        load_gate8(p.og, out_base, lane, gate);
+        apply_output_gate8(acc, p.og, gate, lane, p.io_bf16);
+        store8(p.attn_out, out_base, lane, p.io_bf16, acc);
+    }
 }
 
 // Cross-shard merge: parts is [num_parts][rows][258]; one warp per row.
