@@ -206,3 +206,24 @@ def test_a_nan_that_every_row_sees_is_no_standstill(env, name, hq, hkv, lens, ct
     spoiled = _microseconds(call)
     assert torch.isnan(out).any(-1).all()
     assert spoiled < 20 * clean, (clean, spoiled)
+
+
+@pytest.mark.parametrize("name,hq,hkv,lens,ctx,times", [("tq4", 16, 4, [2048], [2048], 110), ("tq4", 8, 2, [100], [20000], 400), ("bf16", 16, 4, [4] * 16, [6000] * 16, 60)])
+def test_a_nan_among_the_new_tokens_is_bounded(env, name, hq, hkv, lens, ctx, times):
+    """One NaN in the V of a token in the middle of the chunk: the rows of its tile that come before it are computed again, key by key, at most
+    128 rows to a CTA.  (Keys one after the other made the first two 186 and 1100 times as long as the call without NaN, now 56 and 150.)"""
+    kv = env["kv"]
+    cache = Cache(name, hkv, lens, ctx, seed=25)
+    q, batch, ex = _queries(name, sum(lens), hq, 26), cache.batch(), kv.Executor(64 << 20)
+    out = torch.zeros_like(q)
+    call = lambda: kv.paged_attention_scored(ex, cache.layer, batch, q, out, hq, softcap=20.0)  # noqa: E731
+    clean = _microseconds(call)
+    first = out.clone()
+    at = lens[0] // 2 + (20 if lens[0] > 50 else 0)
+    _spoil_v(cache, 0, ctx[0] + at, [7])
+    cache.upload()
+    spoiled = _microseconds(call)
+    eps = torch.finfo(q.dtype).eps
+    assert ((out[:at].double() - first[:at].double()).abs() <= 2 * eps * first[:at].double().abs() + 2 * SHARE[name] * 1.2).all()      # two roundings, two shares
+    assert torch.isnan(out[at:lens[0]]).any(-1).all() and not torch.isnan(out[lens[0]:]).any()
+    assert spoiled < times * clean, (clean, spoiled)

@@ -110,9 +110,9 @@ __device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((u
 //   warps 0-7   consumers: two threads a row, each with one half of the keys of either half of a block; their maxima meet in shared memory
 //   warps 8-9   K, warps 10-11 V: rows copied to their swizzled places, 16 bytes a lane (cp.async)
 //   warp 12     as above; the output product of a block's first half starts as soon as that half's weights are there
-//               (both halves at once: 964 instead of 937 us for 4 x 2048 capped tokens after 2048, 24 / 4 heads)
-// What bounds it: capped, the consumers (three special functions a score against one) and the power cap: 8 x 2048 tokens after 8192
-// take 3.3 to 3.5 ms capped and 2.8 ms = 880 TFLOP/s uncapped.
+//               (both halves at once: 3 % longer for 4 x 2048 capped tokens after 2048, 24 / 4 heads, which take 1.1 ms)
+// What bounds it: capped, the consumers (three special functions a score against one) and the power cap: 8 x 2048 tokens after 8192, 16 / 4
+// heads, take 3.2 to 3.5 ms capped and 2.8 to 3.1 ms = 800 to 870 TFLOP/s uncapped, the shorter times one call at a time.
 template <int FMT> struct PpSmem {
     static constexpr bool kDirect = FMT == WARP34_KV_FORMAT_BF16;
     static constexpr int kStages = kDirect ? 4 : kPpStages;
@@ -1303,7 +1303,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPpThreads, 1) atten
                 if (!fits) {
                     if constexpr (SCORED) {
                         const ScoredRow one = {&p.layout, &p.batch, &p.sc, p.q_in, p.io_bf16, p.num_q_heads, p.gqa};
-                        scored_row_keys(one, place[0], q_off, q_head, place[1] << KB, ((place[1] + nblocks) << KB) - 1, 0, 1, v, m, l);
+                        scored_row_keys<1>(one, place[0], q_off, q_head, place[1] << KB, ((place[1] + nblocks) << KB) - 1, 0, 1, v, m, l);
 #pragma unroll
                         for (int i = 0; i < 8; ++i) v[i] *= ROT ? kPpLutScale : 1.0f;
                     } else if constexpr (!DIRECT) {

@@ -3,39 +3,84 @@
 // second look at rows that came out non-finite.  The latter because a product of a tile's weights with its V rows meets every row of
 // the tile with every key of it: a NaN or infinity in the V of a key that one row must not see (another document's, say) is 0 x NaN there.
 // A row that sees every such key itself is what it must be, and is left alone (scored_bad_rows: one look at the keys of its tile, bound by
-// memory.  Computing such rows again, key by key, took 1000 times as long as the call: 74 ms for 2048 BF16 tokens after 2048, 24 / 4 heads,
-// behind one NaN in the prefix).
+// memory.  Computing such rows again, key by key: 74 ms instead of 0.67 for 2048 BF16 tokens after 2048, 24 / 4 heads, behind one NaN in the
+// prefix; 0.32 without it).
 // Included by tq4_attention.cu.
 #pragma once
 
 namespace w34 {
 
-// Columns [8 lane, + 8) of a stored row (TQ4: in the rotated basis).
-__device__ __forceinline__ void scored_elements(const uint8_t* row, int format, int lane, float (&x)[8]) {
+// A stored row's columns [8 lane, + 8) as they lie in memory (TQ4: in the rotated basis), so that several rows are on their way before the
+// first is used.
+struct ScoredRaw { uint32_t w[4]; float d; };
+__device__ __forceinline__ void scored_load(ScoredRaw& r, const uint8_t* row, int format, int lane, int aligned) {
     if (format == WARP34_KV_FORMAT_TQ4) {
         const uint8_t* half = row + kTq4BlockBytes * (lane >> 4);
         const uint16_t* codes = reinterpret_cast<const uint16_t*>(half + 2 + 4 * (lane & 15));
-        const float d = __half2float(*reinterpret_cast<const __half*>(half));
-        const uint32_t w = (uint32_t)codes[0] | ((uint32_t)codes[1] << 16);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = d * tq4_centroid((int)((w >> (4 * i)) & 15u));
+        r.w[0] = codes[0];
+        r.w[1] = codes[1];
+        r.w[2] = *reinterpret_cast<const uint16_t*>(half);
     } else if (format == WARP34_KV_FORMAT_BF16) {
         const uint16_t* src = reinterpret_cast<const uint16_t*>(row) + 8 * lane;
+        if (aligned) {
+            const uint4 q = *reinterpret_cast<const uint4*>(src);
+            r.w[0] = q.x; r.w[1] = q.y; r.w[2] = q.z; r.w[3] = q.w;
+        } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = __uint_as_float((uint32_t)src[i] << 16);
+            for (int i = 0; i < 4; ++i) r.w[i] = (uint32_t)src[2 * i] | ((uint32_t)src[2 * i + 1] << 16);
+        }
     } else {
         const bool fp8 = format == WARP34_KV_FORMAT_FP8_E4M3;
         const uint32_t* codes = reinterpret_cast<const uint32_t*>(row + (fp8 ? 8 * lane : 68 * (lane >> 3) + 4 + 8 * (lane & 7)));
-        const float d = *reinterpret_cast<const float*>(row + (fp8 ? kHeadDim + 4 * (lane >> 4) : 68 * (lane >> 3)));
+        r.w[0] = codes[0];
+        r.w[1] = codes[1];
+        r.d = *reinterpret_cast<const float*>(row + (fp8 ? kHeadDim + 4 * (lane >> 4) : 68 * (lane >> 3)));
+    }
+}
+// `centroid`: of a code; every lane of the warp comes here.
+template <class Centroid>
+__device__ __forceinline__ void scored_values(const ScoredRaw& r, int format, Centroid centroid, float (&x)[8]) {
+    if (format == WARP34_KV_FORMAT_TQ4) {
+        const float d = __half2float(__ushort_as_half((unsigned short)r.w[2]));
+        const uint32_t w = r.w[0] | (r.w[1] << 16);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = d * centroid((w >> (4 * i)) & 15u);
+    } else if (format == WARP34_KV_FORMAT_BF16) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            x[2 * i] = __uint_as_float(r.w[i] << 16);
+            x[2 * i + 1] = __uint_as_float(r.w[i] & 0xffff0000u);
+        }
+    } else {
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             uint32_t a, b;
-            if (fp8) kv8x4_to_f16x4<WARP34_KV_FORMAT_FP8_E4M3>(codes[i], a, b);
-            else kv8x4_to_f16x4<WARP34_KV_FORMAT_Q8_0>(codes[i], a, b);
+            if (format == WARP34_KV_FORMAT_FP8_E4M3) kv8x4_to_f16x4<WARP34_KV_FORMAT_FP8_E4M3>(r.w[i], a, b);
+            else kv8x4_to_f16x4<WARP34_KV_FORMAT_Q8_0>(r.w[i], a, b);
             const float2 fa = __half22float2(*reinterpret_cast<const __half2*>(&a)), fb = __half22float2(*reinterpret_cast<const __half2*>(&b));
-            x[4 * i] = d * fa.x; x[4 * i + 1] = d * fa.y; x[4 * i + 2] = d * fb.x; x[4 * i + 3] = d * fb.y;
+            x[4 * i] = r.d * fa.x; x[4 * i + 1] = r.d * fa.y; x[4 * i + 2] = r.d * fb.x; x[4 * i + 3] = r.d * fb.y;
         }
     }
+}
+
+// Sums over the lanes of N values a lane (a power of two): lane l ends with the sum of value l N / 32.
+template <int N>
+__device__ __forceinline__ float scored_sums(float (&v)[N], int lane) {
+    int step = 16;
+#pragma unroll
+    for (int n = N; n > 1; n >>= 1) {
+        const bool upper = (lane & step) != 0;
+#pragma unroll
+        for (int i = 0; i < n / 2; ++i) {
+            const float keep = upper ? v[i + n / 2] : v[i], give = upper ? v[i] : v[i + n / 2];
+            v[i] = keep + __shfl_xor_sync(0xffffffffu, give, step);
+        }
+        step >>= 1;
+    }
+    float s = v[0];
+#pragma unroll
+    for (int d = 16 / N; d > 0; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
+    return s;
 }
 
 struct ScoredRow {
@@ -46,8 +91,12 @@ struct ScoredRow {
     int io_bf16, num_q_heads, gqa;
 };
 
-// Keys first, first + step, ... of [lo, hi] of one query row by one warp: columns [8 lane, + 8) of sum w V (stored basis), running
-// maximum (log2 units) and mass.
+// Every `step`th group of KEYS keys, from the `first` on, of [lo, hi] of one query row by one warp: columns [8 lane, + 8) of sum w V (stored
+// basis), running maximum (log2 units) and mass.  The keys' rows are on their way at once and their products summed over the lanes
+// together, a key's score to 32 / KEYS lanes (keys one after the other: 1 us a key, on TQ4 with its table in constant memory 4).
+// Four keys where registers allow (0.4 us a key and warp with 14 warps an SM), two in the merge kernel, whose registers bound its blocks an SM, one
+// where it stands inside the chunk kernel (with four there, 8 x 2048 TQ4 tokens after 8192 took 0.6 % longer without coming here).
+template <int KEYS>
 __device__ __forceinline__ void scored_row_keys(const ScoredRow& p, int req, int q_off, int q_head, int lo, int hi, int first, int step, float (&acc)[8],
                                              float& m, float& l) {
     const int lane = threadIdx.x & 31, kv_head = q_head / p.gqa;
@@ -57,6 +106,8 @@ __device__ __forceinline__ void scored_row_keys(const ScoredRow& p, int req, int
     const int32_t* blocks = b.block_tables + (size_t)req * b.max_blocks_per_req;
     const uint8_t* k_head = (const uint8_t*)(uintptr_t)lay.k_base + (size_t)kv_head * lay.k_head_stride_bytes;
     const uint8_t* v_head = (const uint8_t*)(uintptr_t)lay.v_base + (size_t)kv_head * lay.v_head_stride_bytes;
+    const int aligned = ((lay.k_base | lay.v_base | lay.k_page_stride_bytes | lay.k_head_stride_bytes | lay.k_token_stride_bytes | lay.v_page_stride_bytes |
+                          lay.v_head_stride_bytes | lay.v_token_stride_bytes) & 15u) == 0u;
     lo = max(lo, row_first_key<true>(b, *p.sc, g, q_off));
     hi = min(hi, row_last_key<true>(b, *p.sc, g, q_off));
     float q[8];
@@ -67,46 +118,62 @@ __device__ __forceinline__ void scored_row_keys(const ScoredRow& p, int req, int
         butterfly8<5>(q, lane);
         scale *= 0.0625f;
     }
-    const float slope = row_slope(*p.sc, q_head);
+    const float slope = row_slope(*p.sc, q_head), mine = tq4_centroid(lane & 15);
+    const auto centroid = [&](uint32_t code) { return __shfl_sync(0xffffffffu, mine, (int)code); };
     const int q_pos = g.ctx_before + q_off;
     m = -1e30f;
     l = 0.0f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) acc[i] = 0.0f;
     if (lo > hi) return;
+    const int last = hi / KEYS;
+    auto page_of = [&](int n) { return n <= last ? block_table_page(blocks, n / (kPageTokens / KEYS), b.max_blocks_per_req, kInScalar) : 0; };
+    int n = lo / KEYS + first, page = page_of(n);
 #pragma unroll 1
-    for (int pos0 = lo + first; pos0 <= hi; pos0 += 2 * step) {
-        const uint8_t* vrow[2];
-        float s[2];
-        bool use[2];
+    for (; n <= last; n += step) {
+        ScoredRaw raw[KEYS];      // K, then V
+        const auto load = [&](const uint8_t* run, size_t token_stride, int format) {
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {      // two keys at a time, so that two rows are on their way
-            use[k] = pos0 + k * step <= hi;
-            const int pos = use[k] ? pos0 + k * step : pos0;
-            const int page = block_table_page(blocks, pos >> 4, b.max_blocks_per_req, kInScalar);
-            const size_t off = pos & 15;
-            float x[8];
-            scored_elements(k_head + (size_t)page * lay.k_page_stride_bytes + off * lay.k_token_stride_bytes, lay.k_format, lane, x);
-            vrow[k] = v_head + (size_t)page * lay.v_page_stride_bytes + off * lay.v_token_stride_bytes;
-            float d = 0.0f;
+            for (int i = 0; i < KEYS; ++i) {      // (keys outside the row's are not looked at)
+                scored_load(raw[i], run + (size_t)(min(max(KEYS * n + i, lo), hi) & 15) * token_stride, format, lane, aligned);
+            }
+        };
+        load(k_head + (size_t)page * lay.k_page_stride_bytes, lay.k_token_stride_bytes, lay.k_format);
+        float s[KEYS], x[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) d = __fmaf_rn(q[i], x[i], d);
-            s[k] = warp_sum(d) * scale;
-            if (p.sc->cap != 0.0f) s[k] = capped_score(*p.sc, s[k]);
-            s[k] = __fmaf_rn(-slope, (float)abs(q_pos - pos), s[k]);
+        for (int i = 0; i < KEYS; ++i) {
+            scored_values(raw[i], lay.k_format, centroid, x);
+            s[i] = 0.0f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) s[i] = __fmaf_rn(q[e], x[e], s[i]);
         }
+        load(v_head + (size_t)page * lay.v_page_stride_bytes, lay.v_token_stride_bytes, lay.v_format);
+        page = page_of(n + step);
+        const int pos = KEYS * n + lane / (32 / KEYS);      // the key whose score ends in this lane
+        const bool seen = pos >= lo && pos <= hi;
+        float t = scored_sums(s, lane) * scale;
+        if (p.sc->cap != 0.0f) t = capped_score(*p.sc, t);
+        t = __fmaf_rn(-slope, (float)abs(q_pos - pos), t);
+        float top = seen ? t : -1e30f;
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-            if (!use[k]) continue;
-            const float m_new = fmaxf(m, s[k]), alpha = ex2(m - m_new), w = ex2(s[k] - m_new);
-            float x[8];
-            scored_elements(vrow[k], lay.v_format, lane, x);
-            l = l * alpha + w;
-            m = m_new;
+        for (int d = 32 / KEYS; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+        const float m_new = fmaxf(m, top), alpha = ex2(m - m_new), w = seen ? ex2(t - m_new) : 0.0f;
+        float sum = w;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) acc[i] = __fmaf_rn(acc[i], alpha, w * x[i]);
-        }
+        for (int d = 32 / KEYS; d < 32; d <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+        m = m_new;
+        l = l * alpha + sum;
         if (l != l) return;      // a NaN in the query or in a key: the row is NaN whatever follows
+#pragma unroll
+        for (int e = 0; e < 8; ++e) acc[e] *= alpha;
+#pragma unroll
+        for (int i = 0; i < KEYS; ++i) {
+            if (KEYS * n + i < lo || KEYS * n + i > hi) continue;
+            const float wi = __shfl_sync(0xffffffffu, w, 32 / KEYS * i);
+            scored_values(raw[i], lay.v_format, centroid, x);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) acc[e] = __fmaf_rn(wi, x[e], acc[e]);
+        }
     }
 }
 
@@ -261,7 +328,7 @@ __device__ __forceinline__ void scored_row_join(float (*s_acc)[kHeadDim], const 
 __device__ __forceinline__ void scored_row_whole(const ScoredRow& p, int req, int q_off, int q_head, void* out) {
     const int lane = threadIdx.x & 31;
     float v[8], m, l;
-    scored_row_keys(p, req, q_off, q_head, 0, 0x7ffffffe, 0, 1, v, m, l);
+    scored_row_keys<4>(p, req, q_off, q_head, 0, 0x7ffffffe, 0, 1, v, m, l);
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     const bool rotated = p.layout->v_format == WARP34_KV_FORMAT_TQ4;
 #pragma unroll
@@ -273,7 +340,7 @@ __device__ __forceinline__ void scored_row_whole(const ScoredRow& p, int req, in
     store8(out, ((size_t)(p.batch->query_start_loc[req] + q_off) * p.num_q_heads + q_head) * kHeadDim, lane, p.io_bf16, v);
 }
 
-// Both as calls, for the chunk kernel: in line they take registers from what is around them.
+// As calls, for the chunk kernel: in line they take registers from what is around them.
 __device__ __noinline__ ScoredBad scored_bad_rows_call(const ScoredRow p, int req, int kv_head, int lo, int hi, int first, int step) {
     return scored_bad_rows(p, req, kv_head, lo, hi, first, step);
 }
@@ -281,7 +348,7 @@ __device__ __noinline__ void scored_row_whole_call(const ScoredRow p, int req, i
     scored_row_whole(p, req, q_off, q_head, out);
 }
 
-// One block of four warps per (token, q head); warp w takes the keys first + w, + 4, ...
+// One block of four warps per (token, q head); warp w takes every fourth group of four keys.
 struct ScoredParams {
     warp34_kv_layer_layout layout;
     warp34_attention_batch batch;
@@ -302,7 +369,7 @@ __global__ void __launch_bounds__(128) scored_rows_kernel(const __grid_constant_
     if (req < 0 || !load_req(p.batch, req).valid) return;
     const ScoredRow row = {&p.layout, &p.batch, &p.sc, p.q_in, p.io_bf16, p.num_q_heads, p.num_q_heads / p.layout.local_kv_heads};
     float acc[8], m, l;
-    scored_row_keys(row, req, tok - p.batch.query_start_loc[req], q_head, 0, 0x7ffffffe, wid, 4, acc, m, l);
+    scored_row_keys<4>(row, req, tok - p.batch.query_start_loc[req], q_head, 0, 0x7ffffffe, wid, 4, acc, m, l);
     *reinterpret_cast<float4*>(&s_acc[wid][8 * lane]) = make_float4(acc[0], acc[1], acc[2], acc[3]);
     *reinterpret_cast<float4*>(&s_acc[wid][8 * lane + 4]) = make_float4(acc[4], acc[5], acc[6], acc[7]);
     if (lane == 0) { s_m[wid] = m; s_l[wid] = l; }

@@ -16,77 +16,6 @@ constexpr int kSmallWarps = 8, kSmallCluster = 8;
 constexpr int kSmallRow = kHeadDim + 4;    // floats of a row's state: 256 columns, maximum, mass
 constexpr int kSmallAhead = 3;             // keys whose rows are on their way
 
-// A stored row's columns [8 lane, + 8) as they lie in memory, so that several rows are on their way before the first is used.
-struct SmallRaw { uint32_t w[4]; float d; };
-__device__ __forceinline__ void small_load(SmallRaw& r, const uint8_t* row, int format, int lane, int aligned) {
-    if (format == WARP34_KV_FORMAT_TQ4) {
-        const uint8_t* half = row + kTq4BlockBytes * (lane >> 4);
-        const uint16_t* codes = reinterpret_cast<const uint16_t*>(half + 2 + 4 * (lane & 15));
-        r.w[0] = codes[0];
-        r.w[1] = codes[1];
-        r.w[2] = *reinterpret_cast<const uint16_t*>(half);
-    } else if (format == WARP34_KV_FORMAT_BF16) {
-        const uint16_t* src = reinterpret_cast<const uint16_t*>(row) + 8 * lane;
-        if (aligned) {
-            const uint4 q = *reinterpret_cast<const uint4*>(src);
-            r.w[0] = q.x; r.w[1] = q.y; r.w[2] = q.z; r.w[3] = q.w;
-        } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) r.w[i] = (uint32_t)src[2 * i] | ((uint32_t)src[2 * i + 1] << 16);
-        }
-    } else {
-        const bool fp8 = format == WARP34_KV_FORMAT_FP8_E4M3;
-        const uint32_t* codes = reinterpret_cast<const uint32_t*>(row + (fp8 ? 8 * lane : 68 * (lane >> 3) + 4 + 8 * (lane & 7)));
-        r.w[0] = codes[0];
-        r.w[1] = codes[1];
-        r.d = *reinterpret_cast<const float*>(row + (fp8 ? kHeadDim + 4 * (lane >> 4) : 68 * (lane >> 3)));
-    }
-}
-// `centroids`: the 16 centroids in shared memory.
-__device__ __forceinline__ void small_values(const SmallRaw& r, int format, const float* centroids, float (&x)[8]) {
-    if (format == WARP34_KV_FORMAT_TQ4) {
-        const float d = __half2float(__ushort_as_half((unsigned short)r.w[2]));
-        const uint32_t w = r.w[0] | (r.w[1] << 16);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = d * centroids[(w >> (4 * i)) & 15u];
-    } else if (format == WARP34_KV_FORMAT_BF16) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            x[2 * i] = __uint_as_float(r.w[i] << 16);
-            x[2 * i + 1] = __uint_as_float(r.w[i] & 0xffff0000u);
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            uint32_t a, b;
-            if (format == WARP34_KV_FORMAT_FP8_E4M3) kv8x4_to_f16x4<WARP34_KV_FORMAT_FP8_E4M3>(r.w[i], a, b);
-            else kv8x4_to_f16x4<WARP34_KV_FORMAT_Q8_0>(r.w[i], a, b);
-            const float2 fa = __half22float2(*reinterpret_cast<const __half2*>(&a)), fb = __half22float2(*reinterpret_cast<const __half2*>(&b));
-            x[4 * i] = r.d * fa.x; x[4 * i + 1] = r.d * fa.y; x[4 * i + 2] = r.d * fb.x; x[4 * i + 3] = r.d * fb.y;
-        }
-    }
-}
-
-// Sums over the lanes of N values a lane (a power of two): lane l ends with the sum of value l N / 32.
-template <int N>
-__device__ __forceinline__ float small_sums(float (&v)[N], int lane) {
-    int step = 16;
-#pragma unroll
-    for (int n = N; n > 1; n >>= 1) {
-        const bool upper = (lane & step) != 0;
-#pragma unroll
-        for (int i = 0; i < n / 2; ++i) {
-            const float keep = upper ? v[i + n / 2] : v[i], give = upper ? v[i] : v[i + n / 2];
-            v[i] = keep + __shfl_xor_sync(0xffffffffu, give, step);
-        }
-        step >>= 1;
-    }
-    float s = v[0];
-#pragma unroll
-    for (int d = 16 / N; d > 0; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
-    return s;
-}
-
 struct SmallParams {
     warp34_kv_layer_layout layout;
     warp34_attention_batch batch;
@@ -128,13 +57,13 @@ __global__ void __cluster_dims__(kSmallCluster, 1, 1) __launch_bounds__(kSmallWa
     const long long keys = (long long)hi - lo + 1;
 
     // The rows of a warp's next keys are on their way while it works on one, and the page of the key behind those.
-    SmallRaw k_ahead[kSmallAhead] = {}, v_ahead[kSmallAhead] = {};
+    ScoredRaw k_ahead[kSmallAhead] = {}, v_ahead[kSmallAhead] = {};
     auto page_of = [&](long long n) { return n < keys ? block_table_page(blocks, (lo + (int)n) >> 4, p.batch.max_blocks_per_req, kInScalar) : 0; };
-    auto load = [&](SmallRaw& k, SmallRaw& v, long long n, int page) {
+    auto load = [&](ScoredRaw& k, ScoredRaw& v, long long n, int page) {
         if (n >= keys) return;
         const size_t off = (size_t)((lo + (int)n) & 15);
-        small_load(k, k_head + (size_t)page * p.layout.k_page_stride_bytes + off * p.layout.k_token_stride_bytes, k_format, lane, p.aligned);
-        small_load(v, v_head + (size_t)page * p.layout.v_page_stride_bytes + off * p.layout.v_token_stride_bytes, v_format, lane, p.aligned);
+        scored_load(k, k_head + (size_t)page * p.layout.k_page_stride_bytes + off * p.layout.k_token_stride_bytes, k_format, lane, p.aligned);
+        scored_load(v, v_head + (size_t)page * p.layout.v_page_stride_bytes + off * p.layout.v_token_stride_bytes, v_format, lane, p.aligned);
     };
     long long n = rank * kSmallWarps + wid;
     int page;
@@ -175,9 +104,10 @@ __global__ void __cluster_dims__(kSmallCluster, 1, 1) __launch_bounds__(kSmallWa
     const int my_row = lane >> (5 - LGP);      // the row whose score ends in this lane
     const float slope = my_row < p.gqa ? row_slope(p.sc, kv_head * p.gqa + my_row) : 0.0f;
     float m = -1e30f, l = 0.0f;      // of my_row
+    const auto centroid = [&](uint32_t code) { return s_centroids[code]; };
 #pragma unroll 1
     for (; n < keys; n += kStep) {
-        const SmallRaw kr = k_ahead[0], vr = v_ahead[0];
+        const ScoredRaw kr = k_ahead[0], vr = v_ahead[0];
 #pragma unroll
         for (int a = 0; a + 1 < kSmallAhead; ++a) {
             k_ahead[a] = k_ahead[a + 1];
@@ -186,14 +116,14 @@ __global__ void __cluster_dims__(kSmallCluster, 1, 1) __launch_bounds__(kSmallWa
         load(k_ahead[kSmallAhead - 1], v_ahead[kSmallAhead - 1], n + kSmallAhead * kStep, page);
         page = page_of(n + (kSmallAhead + 1) * kStep);
         float x[8], s[GP];
-        small_values(kr, k_format, s_centroids, x);
+        scored_values(kr, k_format, centroid, x);
 #pragma unroll
         for (int r = 0; r < GP; ++r) {
             s[r] = 0.0f;
 #pragma unroll
             for (int i = 0; i < 8; ++i) s[r] = __fmaf_rn(q[r][i], x[i], s[r]);
         }
-        const float t = changed_score(p.sc, small_sums(s, lane), slope, (float)(q_pos - (lo + (int)n)));
+        const float t = changed_score(p.sc, scored_sums(s, lane), slope, (float)(q_pos - (lo + (int)n)));
         const float m_new = fmaxf(m, t), alpha = ex2(m - m_new), w = ex2(t - m_new);
         m = m_new;
         l = l * alpha + w;
@@ -205,7 +135,7 @@ __global__ void __cluster_dims__(kSmallCluster, 1, 1) __launch_bounds__(kSmallWa
                 for (int i = 0; i < 8; ++i) acc[r][i] *= a;
             }
         }
-        small_values(vr, v_format, s_centroids, x);
+        scored_values(vr, v_format, centroid, x);
 #pragma unroll
         for (int r = 0; r < GP; ++r) {
             const float wr = __shfl_sync(0xffffffffu, w, r << (5 - LGP));

@@ -1591,7 +1591,7 @@ __global__ void __launch_bounds__(MW * 32, SCORED && MW == 4 ? 7 : 0) tq4_attent
         bad.k_first = s_again[1]; bad.k_last = s_again[2]; bad.v_first = s_again[3]; bad.v_last = s_again[4];
         if (bad.explains(row_first_key<true>(p.batch, p.sc, g, tok - g.q_start), row_last_key<true>(p.batch, p.sc, g, tok - g.q_start))) return;
         float m, l;
-        scored_row_keys(row, r, tok - g.q_start, q_head, 0, 0x7ffffffe, wid, MW, acc, m, l);
+        scored_row_keys<2>(row, r, tok - g.q_start, q_head, 0, 0x7ffffffe, wid, MW, acc, m, l);
         *reinterpret_cast<float4*>(&s_acc[wid][8 * lane]) = make_float4(acc[0], acc[1], acc[2], acc[3]);
         *reinterpret_cast<float4*>(&s_acc[wid][8 * lane + 4]) = make_float4(acc[4], acc[5], acc[6], acc[7]);
         if (lane == 0) { s_m[wid] = m; s_l[wid] = l; }
