@@ -503,7 +503,7 @@ int warp34_qsa_sparse_paged_attn_hadamard_f16(const warp34_exec* ex, const void*
  * full grids; less is served more slowly, none, where the call needs some, by a row-at-a-time fp32 kernel), accuracy, stream, capture.  Masked rows of attn_out are left untouched.
  * The _FAST_ATTENTION and _TCGEN05_VERIFY flags change nothing here, _PRECISE_ATTENTION selects the fp32 kernel.
  * Layers: _f16 TQ4 (any strides), Q8_0 / FP8 E4M3 (K and V each in either); _bf16 BF16 and TQ4; head_dim 256, 16-token pages; anything else
- * returns cudaErrorNotSupported, and so does a softcap outside [2^-10, 1024] (above, a float is too coarse for the cap itself: 2e-4 of
+ * returns cudaErrorNotSupported, and so does a softcap outside [2^-10, 1024] (above, a float is too coarse for the cap itself: 6e-4 of
  * a weight at 1024).  A softcap below 0 or NaN is invalid.  K or V rows with NaN or infinity reach only the rows that see them: such a
  * row comes out NaN or infinite, in the channels that are in the V row; rows that share a tile with one and do not see what it sees are
  * computed a second time, one by one in fp32.  So are rows whose finite values leave fp16's range on the way (queries above 60000, say).

@@ -16,8 +16,10 @@
 // transposed), so that a lane stores 16 bytes.  (With movmatrix instead of that and 8 bytes a lane 124 instructions a row, 23 of them on the shared-memory pipe instead of 12.)
 // (Eight lanes to a row, the transform in packed fp32 arithmetic and its columns changing lanes through shared memory: 67 us instead of
 // 52 for 35065 tokens of 4 heads, at 40 shared-memory wavefronts and 168 instructions a row.)
-// Bound by instruction issue: 119 a row, two thirds of the slots with 24 warps an SM; HBM is at 0.54 of the copy rate.  8-bit and BF16 rows,
-// 0.7 and 0.8 of it.  The rows of a warp's next token are on their way while it computes (57 instead of 61 us with a cold L2; with the
+// What that is off by: an element of Z 2^-25 twice, its sums and X 2^-24 more; U sums eight of them, Y both halves with their scales: 18 x 2^-24
+// (|d0| + |d1|) at most, 2^-24 (|d0| + |d1|) in the root mean square of independent roundings, where a row's values are about (|d0| + |d1|) / 32.
+// Bound by instruction issue: 119 a row, two thirds of the slots with 24 warps an SM; HBM is at 0.54 of the copy rate.  The same 35065 tokens
+// of FP8, Q8_0 and BF16 rows take 45.5, 44.4 and 51.0 us (0.74, 0.77 and 0.87 of it).  The rows of a warp's next token are on their way while it computes (57 instead of 61 us with a cold L2; with the
 // registers of four blocks an SM instead of three they spill).
 #include "tq4_common.cuh"
 
@@ -71,8 +73,9 @@ __device__ __forceinline__ uint32_t read_half2(float a, float b) {
     const __half2 v = __floats2half2_rn(a, b);
     return *reinterpret_cast<const uint32_t*>(&v);
 }
-// a and b as fp16 pairs of values and of residuals.  The value is cut off, not rounded (one instruction, and exactly what the pair then holds):
-// the residual is below 2^-10 of it and keeps 11 bits of its own.
+// a and b as fp16 pairs of values and of residuals.  The value is cut off to fp16's 11 bits, not rounded (one instruction), and exact as fp16 from
+// 2^-14 up; the residual is below 2^-10 of it.  Elements of Z are 1/64 and less than 0.17 in magnitude, so residuals, and values below 2^-14, are in
+// the range of fp16's fixed steps of 2^-24: each is off by 2^-25 at most.
 __device__ __forceinline__ void read_split(float a, float b, uint32_t& value, uint32_t& residual) {
     const float va = __uint_as_float(__float_as_uint(a) & 0xffffe000u), vb = __uint_as_float(__float_as_uint(b) & 0xffffe000u);
     value = read_half2(va, vb);
@@ -142,7 +145,7 @@ __global__ void __launch_bounds__(kReadWarps * 32, kReadTq4Blocks) kv_read_tq4_k
     __shared__ __align__(128) uint8_t table[kReadTableBytes];
     __shared__ __align__(128) uint8_t turns[512 * kReadWarps];
     const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5, gid = lane >> 2, tig = lane & 3;
-    {      // entry `threadIdx.x`; centroids x 16, so that their residuals are normal numbers
+    {      // entry `threadIdx.x`; centroids x 16 (0.13 to 2.7), so that 2^-25, the most by which their residuals are off, is 2^-22 of the smallest
         const float c0 = 16.0f * tq4_centroid(threadIdx.x & 15), c1 = 16.0f * tq4_centroid(threadIdx.x >> 4);
         const uint32_t hi = read_half2(c0, c1);
         const float2 hf = __half22float2(*reinterpret_cast<const __half2*>(&hi));

@@ -9,12 +9,12 @@
 // reference's K half with its two roundings, and appends what it makes; this one is for every layer format and the query half.)
 //
 // A head row is a warp: 8 columns a lane, one 16-byte access each way.  Angles: the frequency becomes turns per position as a
-// 64-bit fraction, whose product with the position wraps modulo one turn by itself; what is left is off by 2^-32 turns and 2^-52 of the
-// whole angle (a product in fp32 is off by 2^-7 rad at position 131072).  Sine and cosine are made once per token and block
+// 64-bit fraction, whose product with the position wraps modulo one turn by itself; what is left is off by 2^-32 turns, 2^-52 of the
+// whole angle and, as a float of up to half a turn, 2^-26 turns = 1e-7 rad (a product in fp32 is off by 2^-7 rad at position 131072).  Sine and cosine are made once per token and block
 // (sincospif) and shared by its heads through shared memory, while the rows are on their way.
 //
-// Bound by HBM: 32768 tokens of 24 query heads with gate and 4 key heads (1745 MB) take 268 us, the measured copy rate; without a gate
-// (940 MB) 222 us, 0.66 of it, half of the issue slots taken.
+// Bound by HBM: on 32768 tokens of 24 query heads with gate and 4 key heads (1745 MB) the kernel takes 268 us, the measured copy rate, and a
+// call among others on changing inputs 295, 0.92 of it; without a gate (940 MB) the kernel takes 221 us, 0.66 of it, half of the issue slots taken.
 #include "tq4_common.cuh"
 
 #include <cuda_bf16.h>

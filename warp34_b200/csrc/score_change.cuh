@@ -4,9 +4,11 @@
 //   key visible iff  first(token) <= position <= last(token)
 //
 // Kernels hold scores in units of log2(e) (weights are powers of two), so the factors here are as well.
-// tanh(x) = 1 - 2 / (e^(2 x) + 1), two special-function instructions: 1.5 x 2^-23 of the cap off at most (sum and reciprocal), which is
-// 2e-4 of a weight at the largest cap that is accepted.  (tanh.approx, one instruction, is off by 2^-11 of the cap: 2.5 % of a weight
-// at a cap of 50.)
+// tanh(x) = 1 - 2 / (e^(2 x) + 1), two special-function instructions, off by less than 5 x 2^-23 of the cap: in units of 2^-23, with
+// u = e^(2 x), the power (2^-22 of itself, and 2^-23 |2 x| from its exponent's rounding) 2 u / (u + 1)^2 (2 + |2 x|), the sum's rounding and the
+// reciprocal 3 / (u + 1), the cap in log2(e) units and the last rounding 1.5 |tanh x|; together 4.8 at most, at 2 x about -3.  That is 6e-4
+// of a weight at the largest cap that is accepted and 3e-5 at a cap of 50.  (tanh.approx, one instruction, is off by 2^-11 of the cap: 2.5 % of a weight at a cap of 50.)
+// A penalty is taken off in fp32: a weight is off by 2^-24 of the largest penalty among the keys that count.
 // Included by tq4_attention.cu.
 #pragma once
 
