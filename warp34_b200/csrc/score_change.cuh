@@ -8,7 +8,8 @@
 // u = e^(2 x), the power (2^-22 of itself, and 2^-23 |2 x| from its exponent's rounding) 2 u / (u + 1)^2 (2 + |2 x|), the sum's rounding and the
 // reciprocal 3 / (u + 1), the cap in log2(e) units and the last rounding 1.5 |tanh x|; together 4.8 at most, at 2 x about -3.  That is 6e-4
 // of a weight at the largest cap that is accepted and 3e-5 at a cap of 50.  (tanh.approx, one instruction, is off by 2^-11 of the cap: 2.5 % of a weight at a cap of 50.)
-// A penalty is taken off in fp32: a weight is off by 2^-24 of the largest penalty among the keys that count.
+// A penalty is taken off in fp32 (its slope in log2(e) units 2 x 2^-24, the score's rounding 2^-24): a weight is off by 3 x 2^-24 of the largest
+// penalty among the keys that count.
 // Included by tq4_attention.cu.
 #pragma once
 
