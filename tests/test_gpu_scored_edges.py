@@ -227,3 +227,22 @@ def test_a_nan_among_the_new_tokens_is_bounded(env, name, hq, hkv, lens, ctx, ti
     assert ((out[:at].double() - first[:at].double()).abs() <= 2 * eps * first[:at].double().abs() + 2 * SHARE[name] * 1.2).all()      # two roundings, two shares
     assert torch.isnan(out[at:lens[0]]).any(-1).all() and not torch.isnan(out[lens[0]:]).any()
     assert spoiled < times * clean, (clean, spoiled)
+
+
+@pytest.mark.parametrize("shape", list(STREAM))
+@pytest.mark.parametrize("name", ["fp8", "q8"])
+def test_8_bit_values_behind_zero_rows(env, name, shape):
+    """The newest keys, which are met first, hold V rows of zeros or next to it, the others ordinary ones; and the other way about."""
+    kv = env["kv"]
+    hq, hkv, lens, ctx = STREAM[shape]
+    for newest, power in ((True, -2000), (True, -130), (False, -2000)):
+        cache = Cache(name, hkv, lens, ctx, seed=14, tail=0xff)
+        powers = np.zeros(cache.rows[1].shape[:3])
+        for r, (c, m) in enumerate(zip(ctx, lens)):
+            pos = np.arange(max(c + m - 37, 0), c + m) if newest else np.arange(0, max(c + m - 37, 0))
+            powers[cache.table[r, pos // 16], :, pos % 16] = power
+        _scale_v(cache, powers)
+        q = _queries(name, sum(lens), hq, 15)
+        out = _attend(kv, kv.Executor(64 << 20), cache, cache.batch(), q, hq, softcap=20.0)
+        want, size = scored_attention(cache, q.float().cpu().numpy(), hq, softcap=20.0)
+        _check(name, out, want, size)
